@@ -77,6 +77,18 @@ void greedy_accept(at::Tensor out, at::Tensor target, at::Tensor draft, at::Tens
 void feed_ids(at::Tensor out, at::Tensor ids, at::Tensor feed, at::Tensor prev, at::Tensor status);
 void kv_push(at::Tensor src_k, at::Tensor src_v, at::Tensor dst_k, at::Tensor dst_v, at::Tensor src_ids,
              at::Tensor dst_ids, at::Tensor status);
+void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                        at::Tensor slots, at::Tensor status);
+void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                       at::Tensor slots, at::Tensor status);
+void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,
+                   at::Tensor k_w, double eps, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                   at::Tensor slots, int64_t nh, at::Tensor status);
+void attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                    at::Tensor cu_q, int64_t nq, at::Tensor k_lens, at::Tensor tables, double scale,
+                    at::Tensor status);
+void step_maps(at::Tensor q_lens, at::Tensor k_lens, at::Tensor ids, int64_t bs, at::Tensor cu, at::Tensor positions,
+               at::Tensor slots, at::Tensor tables, at::Tensor last, at::Tensor status);
 }  // namespace lsb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -125,6 +137,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_bf16_silu_packed", &lsb::gemm_bf16_silu_packed);
   m.def("kv_push", &lsb::kv_push);
   m.def("feed_ids", &lsb::feed_ids);
+  m.def("store_kvcache_int4", &lsb::store_kvcache_int4);
+  m.def("load_kvcache_int4", &lsb::load_kvcache_int4);
+  m.def("qkv_rope_int4", &lsb::qkv_rope_int4);
+  m.def("attention_int4", &lsb::attention_int4);
+  m.def("step_maps", &lsb::step_maps);
   m.def("greedy_accept", &lsb::greedy_accept);
   m.def("gemm_bf16", &lsb::gemm_bf16, py::arg("out"), py::arg("x"), py::arg("w"), py::arg("partials"),
         py::arg("splits"), py::arg("status"), py::arg("max_stages") = 0);

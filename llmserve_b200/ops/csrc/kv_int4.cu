@@ -1,0 +1,367 @@
+// Filling and reading back 4-bit KV pages (format: int4_pages.cuh).
+//
+// All three kernels give a lane eight consecutive dims of a row (one 16-byte access of bf16, one
+// 4-byte word of codes), so a group of 64 dims is eight lanes and its range two three-step butterflies.
+// They move each byte once and are bound by memory for prompts, by launch latency for a step's rows.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "int4_pages.cuh"
+
+namespace lsb {
+
+int* status_ptr(const at::Tensor& status);
+
+namespace {
+
+using namespace int4;
+constexpr int kThreads = 128;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Codes (eight nibbles, dim order) and scale word of a group of 64 held eight values to a lane by
+// eight neighbouring lanes; every lane of the group gets the word.
+//   range widened to hold zero; s = range / 15 rounded UP to four significant bits, so no code
+//   saturates by more than the half step that rounding both ends can cost; z = rint(-min / s);
+//   c = min(15, rint(x / s) + z).
+// A group whose range is below 15 times the smallest normal number is stored as zeros, one that holds
+// an infinity or a NaN as NaN (scale NaN), so that a broken row stays visible.
+//
+// x / s is x * (1 / s): for bf16 inputs (kSnap) a quotient that lies exactly half way between two
+// codes must stay there.  x has eight significant bits and s four, so a quotient above 1/4 that is
+// not half way is at least 2^-6 / 30 = 5.2e-4 away from it; rounding to a multiple of 2^-13 (adding
+// and subtracting 1536) moves it by 6.1e-5 at most and removes the 2e-6 that the reciprocal can add,
+// which gives the division's result for a third of its instructions.
+template <bool kSnap>
+__device__ __forceinline__ uint32_t quantise8(const float* x, uint32_t& word) {
+  float mx = 0.f, mn = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mx = max_nan(mx, x[i]);
+    mn = min_nan(mn, x[i]);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+  }
+  const float r = __fdiv_rn(0.5f * mx - 0.5f * mn, 7.5f);
+  if (!(r <= 3.402823466e38f)) {          // NaN or infinity in the group
+    word = 0x7fc0u;
+    return 0u;
+  }
+  word = 0u;
+  if (r < 1.17549435e-38f) return 0u;
+  const uint32_t sbits = (__float_as_uint(r) + 0xfffffu) & 0x7ff00000u;
+  const float s = __uint_as_float(sbits), inv = __fdiv_rn(1.f, s);
+  const int z = __float2int_rn(kSnap ? __fadd_rn(fmaf(-mn, inv, 1536.f), -1536.f) : -mn * inv);
+  word = (sbits >> 16) | (uint32_t)z;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = __float2int_rn(kSnap ? __fadd_rn(fmaf(x[i], inv, 1536.f), -1536.f) : x[i] * inv) + z;
+    codes |= (uint32_t)min(c, 15) << (4 * i);
+  }
+  return codes;
+}
+
+__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* x) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Row (slot, kv head) of a pool; false for a skipped slot (< 0) or one outside the pool (recorded).
+__device__ __forceinline__ bool page_row(int slot, int64_t num_slots, int nkv, int h, uint32_t bs, int* status,
+                                         size_t& row) {
+  if (slot < 0) return false;
+  if (slot >= num_slots) {
+    record_error(status, kBadIndex);
+    return false;
+  }
+  const uint32_t blk = (uint32_t)slot / bs, off = (uint32_t)slot - blk * bs;
+  row = ((size_t)blk * nkv + h) * bs + off;
+  return true;
+}
+
+// grid.y: 0 = K, 1 = V.  Unit u of 8 dims: (token, head, part) in row-major order.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) store_int4_kernel(
+    const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t kst, int64_t ksh, int64_t vst, int64_t vsh,
+    uint8_t* __restrict__ kc, int16_t* __restrict__ kw, uint8_t* __restrict__ vc, int16_t* __restrict__ vw,
+    const int* __restrict__ slots, int64_t units, int nkv, uint32_t bs, int64_t num_slots, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int kLanes = HD / 8;
+  const bool is_v = blockIdx.y != 0;
+  const int64_t u0 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const bool live = u0 < units;
+  const int64_t u = live ? u0 : units - 1;         // tail lanes take part in the butterflies
+  const uint32_t lane = (uint32_t)u % kLanes;
+  const int64_t th = u / kLanes;
+  const int64_t t = th / nkv;
+  const int h = (int)(th - t * nkv);
+  const bf16* src = is_v ? v + t * vst + h * vsh : k + t * kst + h * ksh;
+  float x[8];
+  unpack_bf16x8(*reinterpret_cast<const uint4*>(src + lane * 8), x);
+  const int slot = slots[t];
+  uint32_t word;
+  const uint32_t codes = quantise8<true>(x, word);
+  size_t row;
+  if (!live || !page_row(slot, num_slots, nkv, h, bs, status, row)) return;
+  reinterpret_cast<uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane] = codes;
+  if (lane % 8 == 0) (is_v ? vw : kw)[row * (HD / kGroup) + lane / 8] = (int16_t)word;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads) load_int4_kernel(
+    bf16* __restrict__ k, bf16* __restrict__ v, const uint8_t* __restrict__ kc, const int16_t* __restrict__ kw,
+    const uint8_t* __restrict__ vc, const int16_t* __restrict__ vw, const int* __restrict__ slots, int64_t units,
+    int nkv, uint32_t bs, int64_t num_slots, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int kLanes = HD / 8;
+  const bool is_v = blockIdx.y != 0;
+  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (u >= units) return;
+  const uint32_t lane = (uint32_t)u % kLanes;
+  const int64_t th = u / kLanes;
+  const int64_t t = th / nkv;
+  const int h = (int)(th - t * nkv);
+  uint4 o = make_uint4(0, 0, 0, 0);
+  size_t row;
+  if (page_row(slots[t], num_slots, nkv, h, bs, status, row)) {
+    const uint32_t c = reinterpret_cast<const uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane];
+    const uint32_t w = (uint16_t)(is_v ? vw : kw)[row * (HD / kGroup) + lane / 8];
+    const float s = word_scale(w);
+    const int z = (int)word_zero(w);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = s * (float)((int)((c >> (4 * i)) & 15u) - z);
+    o = make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+  }
+  *reinterpret_cast<uint4*>((is_v ? v : k) + u * 8) = o;
+}
+
+// One step's projection rows [T, (nh + 2 nkv) * HD] (bf16, or S fp32 split-K planes that are summed
+// here): per-head RMS norm of q and k (optional), rotation, q out as bf16, k and v into the pages.
+// Everything between the load and the one rounding at the end is fp32.  HD / 8 lanes hold a head;
+// the rotation's partner dim (d, d + HD/2) is HD / 16 lanes away.
+template <int HD, bool kPlanes>
+__global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
+    bf16* __restrict__ q_out, const void* __restrict__ qkv, int S, const int64_t* __restrict__ positions,
+    const float* __restrict__ cos_sin, int64_t max_pos, const bf16* __restrict__ q_w, const bf16* __restrict__ k_w,
+    float eps, uint8_t* __restrict__ kc, int16_t* __restrict__ kw, uint8_t* __restrict__ vc, int16_t* __restrict__ vw,
+    const int* __restrict__ slots, int T, int nh, int nkv, uint32_t bs, int64_t num_slots, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int kLanes = HD / 8, kHalf = HD / 2;
+  const int heads = nh + 2 * nkv;
+  const int64_t rows = (int64_t)T * heads;
+  const int64_t r0 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const bool live = r0 < rows;
+  const int64_t r = live ? r0 : rows - 1;          // tail lanes take part in the butterflies
+  const int t = (int)(r / heads), head = (int)(r - (int64_t)t * heads);
+  const int lane = threadIdx.x % kLanes, d0 = lane * 8;
+  float x[8];
+  if constexpr (kPlanes) {
+    const float* p = (const float*)qkv + r * HD + d0;
+    const int64_t plane = rows * HD;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < S; ++s) {
+      const float4 a = *reinterpret_cast<const float4*>(p + s * plane);
+      const float4 b = *reinterpret_cast<const float4*>(p + s * plane + 4);
+      x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w;
+      x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+    }
+  } else {
+    unpack_bf16x8(*reinterpret_cast<const uint4*>((const bf16*)qkv + r * HD + d0), x);
+  }
+  const bool is_v = head >= nh + nkv;
+  const bf16* w = head < nh ? q_w : k_w;
+  if (w != nullptr) {                              // uniform over the grid: both or neither
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!is_v) {
+      const float inv = rsqrtf(ss / HD + eps);
+      float g[8];
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(w + d0), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
+    }
+  }
+  int64_t pos = positions[t];
+  const bool pos_ok = pos >= 0 && pos < max_pos;
+  if (!pos_ok) {                                   // never read outside the table; the row is not stored
+    if (live) record_error(status, kBadIndex);
+    pos = 0;
+  }
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
+  if (!is_v) {
+    const float* cs = cos_sin + pos * HD + (d0 & (kHalf - 1));
+    const float sign = d0 < kHalf ? -1.f : 1.f;    // x1 c - x2 s | x2 c + x1 s
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + i);
+      *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(cs + kHalf + i);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + sign * y[i] * s[i];
+  }
+  uint32_t word;
+  // values that are bf16 already (V of a bf16 projection) take the exact-tie form
+  const uint32_t codes = kPlanes ? quantise8<false>(x, word) : (is_v ? quantise8<true>(x, word) : quantise8<false>(x, word));
+  if (!live) return;
+  if (head < nh) {
+    *reinterpret_cast<uint4*>(q_out + ((int64_t)t * nh + head) * HD + d0) =
+        pos_ok ? make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]))
+               : make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int h = is_v ? head - nh - nkv : head - nh;
+  size_t row;
+  if (!pos_ok || !page_row(slots[t], num_slots, nkv, h, bs, status, row)) return;
+  reinterpret_cast<uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane] = codes;
+  if (lane % 8 == 0) (is_v ? vw : kw)[row * (HD / kGroup) + lane / 8] = (int16_t)word;
+}
+
+inline bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// [T, nkv, hd] rows whose last dim is dense and whose rows start on 16 bytes, else a dense copy
+at::Tensor rows_for_store(const at::Tensor& x) {
+  if (x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && x.stride(0) >= 0 && x.stride(1) >= 0 &&
+      aligned16(x))
+    return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+
+void launch_check(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  LSB_INT4_CHECK(e == cudaSuccess, std::string(what) + " launch failed: " + cudaGetErrorString(e));
+}
+
+}  // namespace
+
+void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                        at::Tensor slots, at::Tensor status) {
+  check_page_pair(kc, kw, vc, vw, k.device());
+  LSB_INT4_CHECK(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 3 &&
+                     v.sizes() == k.sizes() && v.device() == k.device(),
+                 "k and v must be bfloat16 [tokens, kv_heads, head_dim]");
+  LSB_INT4_CHECK(k.size(1) == kc.size(1) && k.size(2) == kc.size(3) * 2, "k / v heads do not match the pages");
+  check_int32(slots, "slot_mapping", 1, k.device());
+  LSB_INT4_CHECK(slots.size(0) == k.size(0), "slot_mapping must hold one slot per token");
+  const int64_t units = k.numel() / 8;
+  if (units == 0) return;
+  LSB_INT4_CHECK(units / kThreads < INT32_MAX, "too many rows for one launch");
+  const at::cuda::CUDAGuard g(k.device());
+  k = rows_for_store(k);
+  v = rows_for_store(v);
+  const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2);
+  auto go = [&](auto kern) {
+    launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (const bf16*)k.data_ptr(),
+               (const bf16*)v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kc.data_ptr<uint8_t>(),
+               kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), slots.data_ptr<int>(), units,
+               (int)kc.size(1), (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
+  };
+  if (k.size(2) == 128) go(store_int4_kernel<128>);
+  else go(store_int4_kernel<64>);
+  launch_check("store_kvcache_int4");
+}
+
+void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                       at::Tensor slots, at::Tensor status) {
+  check_page_pair(kc, kw, vc, vw, k.device());
+  check_int32(slots, "slot_mapping", 1, k.device());
+  LSB_INT4_CHECK(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 3 &&
+                     k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.device() == k.device() &&
+                     k.size(0) == slots.size(0) && k.size(1) == kc.size(1) && k.size(2) == kc.size(3) * 2,
+                 "outputs must be contiguous bfloat16 [slots, kv_heads, head_dim]");
+  const int64_t units = k.numel() / 8;
+  if (units == 0) return;
+  LSB_INT4_CHECK(units / kThreads < INT32_MAX, "too many rows for one launch");
+  const at::cuda::CUDAGuard g(k.device());
+  const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2);
+  auto go = [&](auto kern) {
+    launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (bf16*)k.data_ptr(),
+               (bf16*)v.data_ptr(), kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(),
+               vw.data_ptr<int16_t>(), slots.data_ptr<int>(), units, (int)kc.size(1), (uint32_t)kc.size(2),
+               kc.size(0) * kc.size(2), status_ptr(status));
+  };
+  if (k.size(2) == 128) go(load_int4_kernel<128>);
+  else go(load_int4_kernel<64>);
+  launch_check("load_kvcache_int4");
+}
+
+void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,
+                   at::Tensor k_w, double eps, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                   at::Tensor slots, int64_t nh, at::Tensor status) {
+  const at::Device dev = qkv.device();
+  check_page_pair(kc, kw, vc, vw, dev);
+  const bool planes = qkv.scalar_type() == at::kFloat;
+  const int64_t nkv = kc.size(1), hd = kc.size(3) * 2;
+  LSB_INT4_CHECK((planes ? qkv.dim() == 3 : qkv.dim() == 2 && qkv.scalar_type() == at::kBFloat16) &&
+                     qkv.is_contiguous() && aligned16(qkv),
+                 "qkv must be contiguous bfloat16 [T, width] or float32 planes [S, T, width]");
+  LSB_INT4_CHECK(nh >= 1 && qkv.size(-1) == (nh + 2 * nkv) * hd, "qkv width does not match the heads");
+  const int64_t T = qkv.size(-2), S = planes ? qkv.size(0) : 0;
+  LSB_INT4_CHECK(!planes || S >= 1, "no split-K planes");
+  LSB_INT4_CHECK(q_out.scalar_type() == at::kBFloat16 && q_out.is_contiguous() && q_out.numel() == T * nh * hd &&
+                     q_out.device() == dev,
+                 "q_out must be contiguous bfloat16 [T, heads, head_dim]");
+  LSB_INT4_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous() && positions.numel() == T &&
+                     positions.device() == dev,
+                 "positions must be contiguous int64 [T]");
+  LSB_INT4_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.dim() == 2 &&
+                     cos_sin.size(1) == hd && cos_sin.size(0) >= 1 && aligned16(cos_sin) && cos_sin.device() == dev,
+                 "cos_sin must be contiguous float32 [positions, head_dim]");
+  check_int32(slots, "slot_mapping", 1, dev);
+  LSB_INT4_CHECK(slots.size(0) == T, "slot_mapping must hold one slot per token");
+  LSB_INT4_CHECK((q_w.numel() == 0) == (k_w.numel() == 0), "q and k norm weights go together");
+  for (const at::Tensor* w : {&q_w, &k_w})
+    LSB_INT4_CHECK(w->numel() == 0 || (w->scalar_type() == at::kBFloat16 && w->is_contiguous() && w->numel() == hd &&
+                                       aligned16(*w) && w->device() == dev),
+                   "norm weights must be contiguous bfloat16 [head_dim]");
+  if (T == 0) return;
+  const int64_t per = kThreads / (hd / 8), rows = T * (nh + 2 * nkv);
+  LSB_INT4_CHECK(T < INT32_MAX && rows / per < INT32_MAX, "too many rows for one launch");
+  const at::cuda::CUDAGuard g(dev);
+  auto go = [&](auto kern) {
+    launch_pdl(kern, dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(),
+               (bf16*)q_out.data_ptr(), (const void*)qkv.data_ptr(), (int)S, positions.data_ptr<int64_t>(),
+               cos_sin.data_ptr<float>(), cos_sin.size(0), q_w.numel() ? (const bf16*)q_w.data_ptr() : nullptr,
+               k_w.numel() ? (const bf16*)k_w.data_ptr() : nullptr, (float)eps, kc.data_ptr<uint8_t>(),
+               kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), slots.data_ptr<int>(), (int)T,
+               (int)nh, (int)nkv, (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
+  };
+  if (hd == 128) planes ? go(rope_store_int4_kernel<128, true>) : go(rope_store_int4_kernel<128, false>);
+  else planes ? go(rope_store_int4_kernel<64, true>) : go(rope_store_int4_kernel<64, false>);
+  launch_check("qkv_rope_int4");
+}
+
+}  // namespace lsb
