@@ -87,6 +87,9 @@ void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::T
 void attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                     at::Tensor cu_q, int64_t nq, at::Tensor k_lens, at::Tensor tables, double scale,
                     at::Tensor status);
+void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                           int64_t nq, at::Tensor lens, at::Tensor tables, double scale, at::Tensor part_o,
+                           at::Tensor part_ml, at::Tensor counters, int64_t max_splits, at::Tensor status);
 void step_maps(at::Tensor q_lens, at::Tensor k_lens, at::Tensor ids, int64_t bs, at::Tensor cu, at::Tensor positions,
                at::Tensor slots, at::Tensor tables, at::Tensor last, at::Tensor status);
 }  // namespace lsb
@@ -141,6 +144,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("load_kvcache_int4", &lsb::load_kvcache_int4);
   m.def("qkv_rope_int4", &lsb::qkv_rope_int4);
   m.def("attention_int4", &lsb::attention_int4);
+  m.def("decode_attention_int4", &lsb::decode_attention_int4);
   m.def("step_maps", &lsb::step_maps);
   m.def("greedy_accept", &lsb::greedy_accept);
   m.def("gemm_bf16", &lsb::gemm_bf16, py::arg("out"), py::arg("x"), py::arg("w"), py::arg("partials"),

@@ -1,0 +1,634 @@
+// Decode and verify attention against 4-bit KV pages (format: int4_pages.cuh).
+//
+// The query rows of one KV head (nq new tokens x heads per KV head) are the narrow side of the tensor
+// core products and the keys and head dims the wide one, with mma.sync m16n8k16 and fp32 sums:
+//   S^T [16 keys x 8 rows]  = C_K [16 x HD] Q^T        O^T [16 dims x 8 rows] += (C_V - 8)^T [16 x 16 keys] W^T
+// so a tile of 16 keys costs 8 rows of padding at most (16 from nine rows on).  A tcgen05 tile would
+// need 128 of them.  The operands are the codes themselves: 128 + c is a bf16 with c in its low
+// mantissa bits (one mask-or for two nibbles), and
+//   s = sum_g sk_g (sum_d q_d (128 + c_d) - (128 + zk_g) sum_d q_d)       g: groups of 64 dims
+//   o_d = sum_j w_jg (c_jd - 8) - sum_j w_jg (zv_jg - 8)                   w_jg = p_j sv_jg, rounded to bf16
+// Taking 8 off V's code before the product (exact) keeps the long sum over keys free of an offset that
+// would have to cancel; K's sum has at most HD terms and its offset leaves a score within
+// 2^-15 sum |q| sk.  The one rounding besides the output's is w, the second operand of a bf16 product.
+//
+// A warp's operand layout asks K for pairs of dims (d, d + 4: one 16-bit lane each of a code word) and V
+// for pairs of keys (one PRMT joins the half words of two rows, then the same mask-or): neither needs a
+// shuffle, and the order of dims or keys inside a product is free as long as both operands share it.
+//
+// One producer warp copies 128-key chunks (codes and words of K and V, a contiguous run per page) into
+// a ring with bulk copies; four consumer warps take 32 keys of every chunk and never meet until a
+// segment ends.  Work is the list of (sequence, KV head, chunk), cut into equal contiguous shares over a
+// grid that fills the GPU once, whatever the lengths: lengths are read on the device, so one captured
+// launch serves any batch.  A (sequence, head) that is cut leaves fp32 partials; the block that
+// finishes last merges them in their order (results do not depend on who is last) and resets the
+// counter.  Bound by memory for long contexts, by instruction issue (about 280 for 16 keys a warp) just
+// behind it.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "int4_pages.cuh"
+#include "umma.cuh"
+
+namespace lsb {
+
+int* status_ptr(const at::Tensor& status);
+
+namespace {
+
+using namespace int4;
+using umma::wait_phase;
+
+constexpr int kChunk = 128;               // keys of a ring stage, the unit of work
+constexpr int kWarps = 4;                 // consumer warps
+constexpr int kWarpKeys = kChunk / kWarps;
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr float kRescaleLog2 = 8.f;
+
+template <int HD, int NT>
+struct DecLayout {
+  static constexpr int kGroups = HD / kGroup;
+  static constexpr int kStages = 3;
+  static constexpr int kCodes = kChunk * HD / 2;           // bytes of one tensor's codes in a stage
+  static constexpr int kWords = kChunk * kGroups * 2;
+  static constexpr int kStage = 2 * kCodes + 2 * kWords;
+  static constexpr int kRow = HD + 4;                      // floats of a merge row (padded)
+  static constexpr int kMergeOff = kStages * kStage;
+  static constexpr int kMlOff = kMergeOff + kWarps * 8 * NT * kRow * 4;
+  static constexpr int kBarOff = kMlOff + kWarps * 8 * NT * 8;
+  static constexpr int kBytes = kBarOff + 128;
+};
+
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+// nibbles s and s + 4 of a word as the bf16 pair (128 + low, 128 + high)
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int s) { return ((w >> (4 * s)) & 0x000f000fu) | 0x43004300u; }
+// the same less 136: (c - 8) exactly
+__device__ __forceinline__ uint32_t centred(uint32_t w, int s) {
+  const uint32_t x = nibbles(w, s);
+  uint32_t y;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
+  return y;
+}
+
+struct Args {
+  bf16* out;
+  const bf16* q;
+  Pages kp, vp;
+  const int* lens;
+  const int* tables;
+  float* part_o;
+  float* part_ml;
+  int* counters;
+  int* status;
+  float scale_log2;
+  int width, B, nq, nh, nkv, bs, nblk, max_splits, row_tiles;
+};
+
+__device__ __forceinline__ int key_count(const Args& a, int b) {
+  return max(0, min(a.lens[b], (int)min((int64_t)a.width * a.bs, (int64_t)INT32_MAX - kChunk)));
+}
+__device__ __forceinline__ int chunk_count(const Args& a, int b) { return (key_count(a, b) + kChunk - 1) / kChunk; }
+
+// This block's share [c0, c1) of all chunks and where it starts; the same in every lane of a warp.
+struct Share {
+  int64_t c0, c1, total;
+  int b;             // sequence of chunk c0
+  int64_t before;    // chunks of one head before sequence b
+};
+__device__ __forceinline__ int64_t share_begin(int64_t total, int64_t grid, int64_t i) { return total * i / grid; }
+
+__device__ __forceinline__ Share find_share(const Args& a, int lane, int64_t& grid) {
+  int64_t sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) sum += b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  Share s;
+  s.total = sum * a.nkv;
+  grid = min((int64_t)gridDim.x, s.total);
+  s.c0 = s.c1 = 0;
+  s.b = 0;
+  s.before = 0;
+  if (blockIdx.x >= grid) return s;
+  s.c0 = share_begin(s.total, grid, blockIdx.x);
+  s.c1 = share_begin(s.total, grid, blockIdx.x + 1);
+  const int64_t want = s.c0 / a.nkv;      // the sequence whose per-head chunks hold this one
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int n = b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > want);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      s.b = b0 + l;
+      s.before = base + __shfl_sync(0xffffffffu, incl - n, l);
+      return s;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return s;
+}
+
+// One stretch of chunks of a (sequence, head) inside the share.
+struct Segment {
+  int b, h, keys, chunks;      // the sequence's keys and chunks
+  int first, n;                // chunks [first, first + n) of them
+  int64_t pair0;               // index of the pair's first chunk in the whole list
+};
+__device__ __forceinline__ bool next_segment(const Args& a, Share& s, Segment& g) {
+  if (s.c0 >= s.c1) return false;
+  g.b = s.b;
+  g.keys = key_count(a, g.b);
+  g.chunks = (g.keys + kChunk - 1) / kChunk;
+  const int64_t in_seq = s.c0 - s.before * a.nkv;
+  g.h = (int)(in_seq / g.chunks);
+  g.first = (int)(in_seq - (int64_t)g.h * g.chunks);
+  g.n = (int)min((int64_t)(g.chunks - g.first), s.c1 - s.c0);
+  g.pair0 = s.before * a.nkv + (int64_t)g.h * g.chunks;
+  s.c0 += g.n;
+  if (g.h == a.nkv - 1 && g.first + g.n == g.chunks) {      // on to the next sequence that has keys
+    s.before += g.chunks;
+    ++s.b;
+    while (s.c0 < s.c1 && chunk_count(a, s.b) == 0) ++s.b;
+  }
+  return true;
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
+  using L = DecLayout<HD, NT>;
+  constexpr int kG = L::kGroups, kQ = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + L::kStages;
+  volatile uint32_t* bad_tiles = reinterpret_cast<uint32_t*>(empty + L::kStages);    // a bit per 16 keys of the stage
+  __shared__ int abort_flag;
+  __shared__ int merge_me;
+  volatile int* abort_v = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    fence_barrier_init();
+  }
+  pdl_trigger();
+  pdl_wait();
+  __syncthreads();
+  int64_t grid;
+  Share share = find_share(a, lane, grid);
+  Segment g;
+
+  if (warp == kWarps) {
+    // ---------------- producer ----------------
+    int it = 0;
+    int issued[L::kStages] = {};
+    bool ok = true;
+    while (ok && next_segment(a, share, g)) {
+      const int* table = a.tables + (int64_t)g.b * a.width;
+      for (int c = g.first; ok && c < g.first + g.n; ++c, ++it) {
+        const int s = it % L::kStages, u = it / L::kStages;
+        if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&empty[s], (u - 1) & 1, abort_v, a.status, kTimeoutSmemEmpty));
+        if (!ok) break;
+        // lane i takes the i-th page that the chunk touches; runs are whole 16-key tiles of a page
+        const int k0 = c * kChunk, kend = min(k0 + kChunk, (g.keys + 15) & ~15);
+        const int page = k0 / a.bs + lane;
+        const int from = max(k0, page * a.bs), to = min(kend, (page + 1) * a.bs);
+        const bool mine = lane < kChunk / 16 + 1 && from < to;
+        int blk = 0;
+        bool bad = false;
+        if (mine) {
+          blk = table[page];
+          bad = blk < 0 || blk >= a.nblk;
+          if (bad) record_error(a.status, kBadIndex);
+        }
+        uint32_t flags = 0;
+        if (bad) flags = ((1u << ((to - k0) / 16)) - 1u) & ~((1u << ((from - k0) / 16)) - 1u);
+        flags = __reduce_or_sync(0xffffffffu, flags);
+        const int keys = mine && !bad ? to - from : 0;
+        const int total = __reduce_add_sync(0xffffffffu, keys);
+        if (lane == 0) {
+          bad_tiles[s] = flags;                    // published by the arrival below
+          mbar_expect_tx(&full[s], (uint32_t)total * (HD + 4 * kG));
+        }
+        __syncwarp();
+        if (keys > 0) {
+          const size_t row = ((size_t)blk * a.nkv + g.h) * a.bs + (from - page * a.bs);
+          const uint32_t st = smem_u32(smem) + s * L::kStage;
+          const int at = from - k0;
+          bulk_copy(st + at * (HD / 2), a.kp.codes + row * (HD / 2), keys * (HD / 2), &full[s]);
+          bulk_copy(st + 2 * L::kCodes + at * 2 * kG, a.kp.words + row * kG, keys * 2 * kG, &full[s]);
+          bulk_copy(st + L::kCodes + at * (HD / 2), a.vp.codes + row * (HD / 2), keys * (HD / 2), &full[s]);
+          bulk_copy(st + 2 * L::kCodes + L::kWords + at * 2 * kG, a.vp.words + row * kG, keys * 2 * kG, &full[s]);
+        }
+        issued[s] = u + 1;
+      }
+    }
+    // every copy has landed before the block may end
+    for (int s = 0; s < L::kStages; ++s)
+      if (issued[s] > 0) mbar_wait(&full[s], (issued[s] - 1) & 1);
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int gid = lane >> 2, t4 = lane & 3;
+  const int group_heads = a.nh / a.nkv;
+  const int row0 = blockIdx.y * kQ, rows = min(kQ, a.nq * group_heads - row0);
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeOff);
+  float2* ml = reinterpret_cast<float2*>(smem + L::kMlOff);
+
+  // sequences without keys: zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (key_count(a, b) == 0)
+      for (int i = threadIdx.x; i < a.nkv * rows * (HD / 8); i += kWarps * 32) {
+        const int r = i / (HD / 8) % rows + row0, h = i / (HD / 8) / rows;
+        const size_t at = ((size_t)b * a.nq + r / group_heads) * a.nh + h * group_heads + r % group_heads;
+        *reinterpret_cast<uint4*>(a.out + at * HD + (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
+      }
+
+  int it = 0;
+  bool ok = true;
+  while (next_segment(a, share, g)) {
+    // address of query row r (< rows) of this pair, in rows of HD
+    auto row_of = [&](int r) {
+      r += row0;
+      return ((size_t)g.b * a.nq + r / group_heads) * a.nh + g.h * group_heads + r % group_heads;
+    };
+    // Q^T operand: for group g and half i, dims 64 g + 16 t4 + 8 i + (s, s + 4); row gid of each 8-row tile
+    uint32_t qf[NT][kG][2][4];
+    float qs[NT][kG][2];                           // sum of q over a group for rows 2 t4, 2 t4 + 1
+    int limit[NT][2];                              // keys that these two rows see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool live = n * 8 + gid < rows;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + row_of(live ? n * 8 + gid : 0) * HD);
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint4 v = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
+          qf[n][gr][i][0] = __byte_perm(v.x, v.z, 0x5410);
+          qf[n][gr][i][1] = __byte_perm(v.x, v.z, 0x7632);
+          qf[n][gr][i][2] = __byte_perm(v.y, v.w, 0x5410);
+          qf[n][gr][i][3] = __byte_perm(v.y, v.w, 0x7632);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qs[n][gr][0] = __shfl_sync(0xffffffffu, sum, t4 * 8);
+        qs[n][gr][1] = __shfl_sync(0xffffffffu, sum, t4 * 8 + 4);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = n * 8 + t4 * 2 + e;
+        limit[n][e] = r < rows ? min(g.keys, a.lens[g.b] - a.nq + (row0 + r) / group_heads + 1) : 0;
+      }
+    }
+    // keys below this are seen by every row of the tile
+    const int all_see = min(g.keys, a.lens[g.b] - a.nq + row0 / group_heads + 1);
+
+    float o[NT][kG][4][4];
+    float m[NT][2], l[NT][2], zc[NT][kG][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][gr][j][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) zc[n][gr][e] = 0.f;
+      }
+    }
+
+    for (int c = g.first; c < g.first + g.n; ++c, ++it) {
+      const int s = it % L::kStages;
+      ok = ok && __all_sync(0xffffffffu, wait_phase(&full[s], (it / L::kStages) & 1, abort_v, a.status, kTimeoutTmaFull));
+      if (!ok) break;
+      const uint32_t st = smem_u32(smem) + s * L::kStage;
+      const uint32_t bad = bad_tiles[s];
+#pragma unroll 1
+      for (int tile = 0; tile < kWarpKeys / 16; ++tile) {
+        const int at = warp * kWarpKeys + tile * 16, k0 = c * kChunk + at;
+        if (k0 >= g.keys || ((bad >> (at / 16)) & 1u)) continue;
+        // Row m of the tile is key (m & 8) + ((m & 7) >> 1) + 4 (m & 1): the four rows that the four lanes
+        // of a group read together for V then lie in two bank halves instead of one.
+        const int key_a = (gid >> 1) + 4 * (gid & 1), key_b = key_a + 8;
+        const uint32_t ka = st + (at + key_a) * (HD / 2), kb = ka + 8 * (HD / 2);
+        float sacc[NT][kG][4];
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          const uint2 wa = lds64(ka + gr * 32 + t4 * 8), wb = lds64(kb + gr * 32 + t4 * 8);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sacc[n][gr][e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t xa = i ? wa.y : wa.x, xb = i ? wb.y : wb.x;
+#pragma unroll
+            for (int p = 0; p < 4; p += 2) {
+              const uint32_t a0 = nibbles(xa, p), a1 = nibbles(xb, p), a2 = nibbles(xa, p + 1), a3 = nibbles(xb, p + 1);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_bf16(sacc[n][gr], a0, a1, a2, a3, qf[n][gr][i][p], qf[n][gr][i][p + 1]);
+            }
+          }
+        }
+        // scale words of keys a and b: group 0 in the low half word, group 1 in the high one
+        const uint32_t kw = st + 2 * L::kCodes, vw = kw + L::kWords;
+        float sk[2][kG], zk[2][kG], sv[2][kG], zv[2][kG];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = at + (e ? key_b : key_a);
+          uint32_t x, y;
+          if constexpr (kG == 2) {
+            x = lds32(kw + key * 4);
+            y = lds32(vw + key * 4);
+          } else {
+            x = lds16(kw + key * 2) << 16;
+            y = lds16(vw + key * 2) << 16;
+          }
+#pragma unroll
+          for (int gr = 0; gr < kG; ++gr) {
+            const uint32_t xw = kG == 2 && gr == 0 ? x << 16 : x, yw = kG == 2 && gr == 0 ? y << 16 : y;
+            sk[e][gr] = __uint_as_float(xw & 0x7ff00000u) * a.scale_log2;
+            zk[e][gr] = __uint_as_float((xw & 0x000f0000u) | 0x43000000u);          // 128 + z
+            sv[e][gr] = __uint_as_float(yw & 0x7ff00000u);
+            zv[e][gr] = __uint_as_float((yw & 0x000f0000u) | 0x43000000u) - 136.f;  // z - 8
+          }
+        }
+        const bool edge = k0 + 16 > all_see;
+        float p[NT][4];                            // [key a row 0, key a row 1, key b row 0, key b row 1]
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < kG; ++gr)
+              x = fmaf(sk[e >> 1][gr], fmaf(-zk[e >> 1][gr], qs[n][gr][e & 1], sacc[n][gr][e]), x);
+            if (edge && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) x = -INFINITY;
+            p[n][e] = x;
+            grow |= x > m[n][e & 1] + kRescaleLog2;
+          }
+        // the reference maximum moves only when a score passes it by 2^8 (first tile: from -inf)
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(p[n][e], p[n][e + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              const float mn = fmaxf(m[n][e], mx), f = m[n][e] == -INFINITY ? 0.f : umma::ex2(m[n][e] - mn);
+              m[n][e] = mn;
+              l[n][e] *= f;
+#pragma unroll
+              for (int gr = 0; gr < kG; ++gr) {
+                zc[n][gr][e] *= f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][gr][j][e] *= f, o[n][gr][j][e + 2] *= f;
+              }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float mm = m[n][e & 1];
+            p[n][e] = umma::ex2(p[n][e] - (mm == -INFINITY ? 0.f : mm));
+            l[n][e & 1] += p[n][e];
+          }
+        // O^T: words of keys (rows 2 t4, 2 t4 + 1, + 8) for dims 64 g + 8 gid ..
+        const uint32_t v0 = st + L::kCodes + (at + t4) * (HD / 2) + gid * 4;
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          uint32_t w0[NT], w1[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[e] = p[n][e] * sv[e >> 1][gr];
+              // a key that this row does not see may hold anything, NaN scales among it
+              if (edge && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) w[e] = 0.f;
+            }
+            const uint32_t lo = umma::pack2_bf16(w[0], w[1]), hi = umma::pack2_bf16(w[2], w[3]);
+            zc[n][gr][0] = fmaf(__uint_as_float(lo << 16), zv[0][gr], fmaf(__uint_as_float(hi << 16), zv[1][gr], zc[n][gr][0]));
+            zc[n][gr][1] = fmaf(__uint_as_float(lo & 0xffff0000u), zv[0][gr],
+                                fmaf(__uint_as_float(hi & 0xffff0000u), zv[1][gr], zc[n][gr][1]));
+            w0[n] = transpose8x8(lo);
+            w1[n] = transpose8x8(hi);
+          }
+          const uint32_t va = v0 + gr * 32;        // row 2 t4 is key t4, row 2 t4 + 1 key t4 + 4
+          const uint32_t x0 = lds32(va), x1 = lds32(va + 4 * (HD / 2)), x8 = lds32(va + 8 * (HD / 2)),
+                         x9 = lds32(va + 12 * (HD / 2));
+          const uint32_t lo01 = __byte_perm(x0, x1, 0x5410), hi01 = __byte_perm(x0, x1, 0x7632);
+          const uint32_t lo89 = __byte_perm(x8, x9, 0x5410), hi89 = __byte_perm(x8, x9, 0x7632);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a0 = centred(lo01, j), a1 = centred(hi01, j), a2 = centred(lo89, j), a3 = centred(hi89, j);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[n][gr][j], a0, a1, a2, a3, w0[n], w1[n]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(&empty[s]);
+    }
+
+    // ---- the warps' results of this segment meet in shared memory ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = n * 8 + t4 * 2 + e;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        if (gid == 0) ml[warp * kQ + r] = make_float2(m[n][e], l[n][e]);
+#pragma unroll
+        for (int gr = 0; gr < kG; ++gr) {
+          float z = zc[n][gr][e];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+          float* dst = merge + (warp * kQ + r) * L::kRow + gr * 64 + gid * 8;
+          *reinterpret_cast<float4*>(dst) = make_float4(o[n][gr][0][e] - z, o[n][gr][1][e] - z, o[n][gr][2][e] - z, o[n][gr][3][e] - z);
+          *reinterpret_cast<float4*>(dst + 4) =
+              make_float4(o[n][gr][0][e + 2] - z, o[n][gr][1][e + 2] - z, o[n][gr][2][e + 2] - z, o[n][gr][3][e + 2] - z);
+        }
+      }
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    const bool whole = g.n == g.chunks;
+    for (int i = threadIdx.x; i < rows * (HD / 8); i += kWarps * 32) {
+      const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
+      float mx = -INFINITY, sum = 0.f, acc[8] = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * kQ + r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 x = ml[w * kQ + r];
+        const float f = x.x == -INFINITY ? 0.f : umma::ex2(x.x - mx);
+        sum += f * x.y;
+        const float* src = merge + (w * kQ + r) * L::kRow + d;
+        if (f != 0.f)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += f * src[e];
+      }
+      const size_t row = row_of(r);
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint4*>(a.out + row * HD + d) =
+            make_uint4(umma::pack2_bf16(acc[0] * inv, acc[1] * inv), umma::pack2_bf16(acc[2] * inv, acc[3] * inv),
+                       umma::pack2_bf16(acc[4] * inv, acc[5] * inv), umma::pack2_bf16(acc[6] * inv, acc[7] * inv));
+      } else {
+        const size_t slot = row * a.max_splits + g.first;
+        float4* dst = reinterpret_cast<float4*>(a.part_o + slot * HD + d);
+        __stcg(dst, make_float4(acc[0], acc[1], acc[2], acc[3]));
+        __stcg(dst + 1, make_float4(acc[4], acc[5], acc[6], acc[7]));
+        if (d == 0) __stcg(reinterpret_cast<float2*>(a.part_ml) + slot, make_float2(mx, sum));
+      }
+    }
+    if (!whole) {
+      // pieces of this pair: cut where the shares of the blocks begin
+      const int64_t i0 = ((g.pair0 + 1) * grid - 1) / share.total;
+      const int64_t i1 = ((g.pair0 + g.chunks) * grid - 1) / share.total;
+      const int pieces = (int)(i1 - i0) + 1;
+      __threadfence();
+      asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+      if (threadIdx.x == 0)
+        merge_me = atomicInc(reinterpret_cast<unsigned*>(a.counters) + ((size_t)g.b * a.nkv + g.h) * a.row_tiles + blockIdx.y,
+                             (unsigned)pieces - 1u) == (unsigned)pieces - 1u;
+      asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+      if (merge_me) {
+        __threadfence();
+        for (int i = threadIdx.x; i < rows * (HD / 8); i += kWarps * 32) {
+          const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
+          const size_t row = row_of(r);
+          float mx = -INFINITY, sum = 0.f, acc[8] = {};
+          for (int x = 0; x < pieces; ++x) {
+            const int first = (int)(max(g.pair0, share_begin(share.total, grid, i0 + x)) - g.pair0);
+            const size_t slot = row * a.max_splits + first;
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot);
+            if (v.y == 0.f) continue;              // saw no key
+            const float mn = fmaxf(mx, v.x), f = mx == -INFINITY ? 0.f : umma::ex2(mx - mn), fx = umma::ex2(v.x - mn);
+            mx = mn;
+            sum = sum * f + fx * v.y;
+            const float4* src = reinterpret_cast<const float4*>(a.part_o + slot * HD + d);
+            const float4 y0 = __ldcg(src), y1 = __ldcg(src + 1);
+            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f + fx * y[e];
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint4*>(a.out + row * HD + d) =
+              make_uint4(umma::pack2_bf16(acc[0] * inv, acc[1] * inv), umma::pack2_bf16(acc[2] * inv, acc[3] * inv),
+                         umma::pack2_bf16(acc[4] * inv, acc[5] * inv), umma::pack2_bf16(acc[6] * inv, acc[7] * inv));
+        }
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");    // the merge rows are free again
+  }
+}
+
+}  // namespace
+
+void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                           int64_t nq, at::Tensor lens, at::Tensor tables, double scale, at::Tensor part_o,
+                           at::Tensor part_ml, at::Tensor counters, int64_t max_splits, at::Tensor status) {
+  const at::Device dev = q.device();
+  check_page_pair(kc, kw, vc, vw, dev);
+  LSB_INT4_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
+                     reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+                 "q must be contiguous, 16-byte aligned bfloat16 [rows, heads, head_dim]");
+  LSB_INT4_CHECK(q.size(2) == kc.size(3) * 2 && q.size(1) >= 1 && q.size(1) % kc.size(1) == 0,
+                 "query heads do not match the pages");
+  LSB_INT4_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous() &&
+                     out.device() == dev, "bad output");
+  check_int32(lens, "sequence lengths", 1, dev);
+  check_int32(tables, "block_tables", 2, dev);
+  const int64_t B = lens.size(0), T = q.size(0), nh = q.size(1), nkv = kc.size(1), hd = q.size(2), bs = kc.size(2);
+  LSB_INT4_CHECK(tables.size(0) >= B, "block_tables must hold one row per sequence");
+  LSB_INT4_CHECK(nq >= 1 && T == B * nq, "q must hold nq rows per sequence");
+  if (T == 0) return;
+  const int64_t cap = tables.size(1) * bs;
+  LSB_INT4_CHECK(part_o.scalar_type() == at::kFloat && part_ml.scalar_type() == at::kFloat &&
+                     counters.scalar_type() == at::kInt && part_o.is_contiguous() && part_ml.is_contiguous() &&
+                     counters.is_contiguous() && part_o.device() == dev && part_ml.device() == dev &&
+                     counters.device() == dev && max_splits * kChunk >= cap && part_o.numel() >= T * nh * max_splits * hd &&
+                     part_ml.numel() >= T * nh * max_splits * 2 && counters.numel() >= T * nh,
+                 "decode workspace too small for this batch");
+  LSB_INT4_CHECK(T * nh < INT32_MAX && nq * (nh / nkv) <= 16 * 65535, "batch exceeds int32 rows");
+  const at::cuda::CUDAGuard guard(dev);
+  const int rows = (int)(nq * (nh / nkv)), nt = rows > 8 ? 2 : 1, tiles = (rows + 8 * nt - 1) / (8 * nt);
+  Args a = {(bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), {kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
+            {vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, lens.data_ptr<int>(), tables.data_ptr<int>(),
+            part_o.data_ptr<float>(), part_ml.data_ptr<float>(), counters.data_ptr<int>(), status_ptr(status),
+            (float)(scale * 1.4426950408889634), (int)tables.size(1), (int)B, (int)nq, (int)nh, (int)nkv, (int)bs,
+            (int)kc.size(0), (int)max_splits, tiles};
+  auto go = [&](auto kern, int smem, int per_sm) {
+    ensure_dynamic_smem((const void*)kern, smem);
+    // as many blocks as fit the GPU at once, shared by the row tiles, and no more than there can be chunks
+    const int64_t most = B * nkv * std::max<int64_t>(1, (cap + kChunk - 1) / kChunk);
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(most, 148 * per_sm / tiles));
+    launch_pdl(kern, dim3((unsigned)grid, tiles), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(), a);
+  };
+#define LSB_DEC(HD, NT, PER) go(decode_int4_kernel<HD, NT>, DecLayout<HD, NT>::kBytes, PER)
+  if (hd == 128) {
+    if (nt == 1) LSB_DEC(128, 1, 3);
+    else LSB_DEC(128, 2, 2);
+  } else {
+    if (nt == 1) LSB_DEC(64, 1, 4);
+    else LSB_DEC(64, 2, 3);
+  }
+#undef LSB_DEC
+  const cudaError_t e = cudaGetLastError();
+  LSB_INT4_CHECK(e == cudaSuccess, std::string("decode_attention_int4 launch failed: ") + cudaGetErrorString(e));
+}
+
+}  // namespace lsb

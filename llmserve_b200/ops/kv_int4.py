@@ -200,16 +200,23 @@ def qkv_norm_rope_store_int4(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, k
 def verify_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_tables, seqlens_k, scale, nq: int,
                           workspace=None):
     """Causal attention of ``nq`` consecutive new tokens per sequence (``q [B * nq, nh, hd]``, sequence
-    b's at positions ``seqlens_k[b] - nq ..``)."""
+    b's at positions ``seqlens_k[b] - nq ..``).  ``workspace``: a ``DecodeWorkspace`` for at least
+    ``B * nq`` rows and the keys that the block tables can address, which calls (and captured graphs) on
+    one stream may share; calls that can overlap need one each.  Without one the call makes its own."""
     if nq < 1 or q.shape[0] != seqlens_k.shape[0] * nq:
         raise ValueError("q must hold nq >= 1 rows per sequence")
     if not q.is_cuda:
         _check_pages(k_pages, v_pages, None, None)
         cu = torch.arange(0, q.shape[0] + 1, nq, dtype=torch.int32)
         return attention_int4_ref(q, k_pages, v_pages, cu, seqlens_k, block_tables, scale)
+    rows, nh, hd = q.shape
+    cap = block_tables.shape[-1] * k_pages.codes.shape[2]
+    if workspace is None or workspace.max_batch < rows or workspace.max_splits * 128 < cap:
+        workspace = attn_ops.DecodeWorkspace(rows, nh, hd, cap, q.device)
     out = torch.empty_like(q)
-    C().attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, seqlens_k, nq,
-                       seqlens_k, block_tables, scale, status(q.device))
+    C().decode_attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, nq,
+                              seqlens_k, block_tables, scale, workspace.partial_out, workspace.partial_ml,
+                              workspace.counters, workspace.max_splits, status(q.device))
     return out
 
 
