@@ -28,6 +28,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <type_traits>
+
 #include "int4_pages.cuh"
 #include "umma.cuh"
 
@@ -50,6 +52,7 @@ template <int HD, int NT>
 struct DecLayout {
   static constexpr int kGroups = HD / kGroup;
   static constexpr int kStages = 3;
+  static constexpr int kBlocks = NT == 2 ? 2 : 3;          // resident blocks per SM that registers are held to
   static constexpr int kCodes = kChunk * HD / 2;           // bytes of one tensor's codes in a stage
   static constexpr int kWords = kChunk * kGroups * 2;
   static constexpr int kStage = 2 * kCodes + 2 * kWords;
@@ -122,41 +125,37 @@ __device__ __forceinline__ int chunk_count(const Args& a, int b) { return (key_c
 
 // This block's share [c0, c1) of all chunks and where it starts; the same in every lane of a warp.
 struct Share {
-  int64_t c0, c1, total;
+  int c0, c1, total;
   int b;             // sequence of chunk c0
-  int64_t before;    // chunks of one head before sequence b
+  int before;        // chunks of all heads before sequence b
 };
-__device__ __forceinline__ int64_t share_begin(int64_t total, int64_t grid, int64_t i) { return total * i / grid; }
+__device__ __forceinline__ int share_begin(int total, int grid, int i) { return (int)((int64_t)total * i / grid); }
 
-__device__ __forceinline__ Share find_share(const Args& a, int lane, int64_t& grid) {
-  int64_t sum = 0;
+__device__ __forceinline__ Share find_share(const Args& a, int lane, int& grid) {
+  int sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) sum += b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   Share s;
-  s.total = sum * a.nkv;
-  grid = min((int64_t)gridDim.x, s.total);
-  s.c0 = s.c1 = 0;
-  s.b = 0;
-  s.before = 0;
-  if (blockIdx.x >= grid) return s;
+  s.total = __reduce_add_sync(0xffffffffu, sum) * a.nkv;
+  grid = min((int)gridDim.x, s.total);
+  s.c0 = s.c1 = s.b = s.before = 0;
+  if ((int)blockIdx.x >= grid) return s;
   s.c0 = share_begin(s.total, grid, blockIdx.x);
   s.c1 = share_begin(s.total, grid, blockIdx.x + 1);
-  const int64_t want = s.c0 / a.nkv;      // the sequence whose per-head chunks hold this one
-  int64_t base = 0;
+  const int want = s.c0 / a.nkv;          // the sequence whose per-head chunks hold this one
+  int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int n = b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
-    int64_t incl = n;
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += u;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > want);
     if (hit) {
       const int l = __ffs(hit) - 1;
       s.b = b0 + l;
-      s.before = base + __shfl_sync(0xffffffffu, incl - n, l);
+      s.before = (base + __shfl_sync(0xffffffffu, incl - n, l)) * a.nkv;
       return s;
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
@@ -168,21 +167,20 @@ __device__ __forceinline__ Share find_share(const Args& a, int lane, int64_t& gr
 struct Segment {
   int b, h, keys, chunks;      // the sequence's keys and chunks
   int first, n;                // chunks [first, first + n) of them
-  int64_t pair0;               // index of the pair's first chunk in the whole list
+  int pair0;                   // index of the pair's first chunk in the whole list
 };
 __device__ __forceinline__ bool next_segment(const Args& a, Share& s, Segment& g) {
   if (s.c0 >= s.c1) return false;
   g.b = s.b;
   g.keys = key_count(a, g.b);
   g.chunks = (g.keys + kChunk - 1) / kChunk;
-  const int64_t in_seq = s.c0 - s.before * a.nkv;
-  g.h = (int)(in_seq / g.chunks);
-  g.first = (int)(in_seq - (int64_t)g.h * g.chunks);
-  g.n = (int)min((int64_t)(g.chunks - g.first), s.c1 - s.c0);
-  g.pair0 = s.before * a.nkv + (int64_t)g.h * g.chunks;
+  g.h = (s.c0 - s.before) / g.chunks;
+  g.pair0 = s.before + g.h * g.chunks;
+  g.first = s.c0 - g.pair0;
+  g.n = min(g.chunks - g.first, s.c1 - s.c0);
   s.c0 += g.n;
   if (g.h == a.nkv - 1 && g.first + g.n == g.chunks) {      // on to the next sequence that has keys
-    s.before += g.chunks;
+    s.before = s.c0;
     ++s.b;
     while (s.c0 < s.c1 && chunk_count(a, s.b) == 0) ++s.b;
   }
@@ -190,7 +188,7 @@ __device__ __forceinline__ bool next_segment(const Args& a, Share& s, Segment& g
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_int4_kernel(const Args a) {
   using L = DecLayout<HD, NT>;
   constexpr int kG = L::kGroups, kQ = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -212,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
   pdl_trigger();
   pdl_wait();
   __syncthreads();
-  int64_t grid;
+  int grid;
   Share share = find_share(a, lane, grid);
   Segment g;
 
@@ -328,7 +326,8 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
     const int all_see = min(g.keys, a.lens[g.b] - a.nq + row0 / group_heads + 1);
 
     float o[NT][kG][4][4];
-    float m[NT][2], l[NT][2], zc[NT][kG][2];
+    // m: the reference that exponents are taken from, top: the score that moves it (-inf: none seen yet)
+    float m[NT][2], top[NT][2], l[NT][2], zc[NT][kG][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -339,7 +338,8 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
           for (int e = 0; e < 4; ++e) o[n][gr][j][e] = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
+        m[n][e] = 0.f;
+        top[n][e] = -INFINITY;
         l[n][e] = 0.f;
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) zc[n][gr][e] = 0.f;
@@ -352,10 +352,9 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
       if (!ok) break;
       const uint32_t st = smem_u32(smem) + s * L::kStage;
       const uint32_t bad = bad_tiles[s];
-#pragma unroll 1
-      for (int tile = 0; tile < kWarpKeys / 16; ++tile) {
-        const int at = warp * kWarpKeys + tile * 16, k0 = c * kChunk + at;
-        if (k0 >= g.keys || ((bad >> (at / 16)) & 1u)) continue;
+      // 16 keys; edge: some row of this block does not see some of them
+      auto tile = [&](auto edge, int at) {
+        const int k0 = c * kChunk + at;
         // Row m of the tile is key (m & 8) + ((m & 7) >> 1) + 4 (m & 1): the four rows that the four lanes
         // of a group read together for V then lie in two bank halves instead of one.
         const int key_a = (gid >> 1) + 4 * (gid & 1), key_b = key_a + 8;
@@ -402,7 +401,6 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
             zv[e][gr] = __uint_as_float((yw & 0x000f0000u) | 0x43000000u) - 136.f;  // z - 8
           }
         }
-        const bool edge = k0 + 16 > all_see;
         float p[NT][4];                            // [key a row 0, key a row 1, key b row 0, key b row 1]
         bool grow = false;
 #pragma unroll
@@ -413,9 +411,9 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
 #pragma unroll
             for (int gr = 0; gr < kG; ++gr)
               x = fmaf(sk[e >> 1][gr], fmaf(-zk[e >> 1][gr], qs[n][gr][e & 1], sacc[n][gr][e]), x);
-            if (edge && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) x = -INFINITY;
+            if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) x = -INFINITY;
             p[n][e] = x;
-            grow |= x > m[n][e & 1] + kRescaleLog2;
+            grow |= x > top[n][e & 1];
           }
         // the reference maximum moves only when a score passes it by 2^8 (first tile: from -inf)
         if (__any_sync(0xffffffffu, grow)) {
@@ -426,8 +424,11 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
               float mx = fmaxf(p[n][e], p[n][e + 2]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              const float mn = fmaxf(m[n][e], mx), f = m[n][e] == -INFINITY ? 0.f : umma::ex2(m[n][e] - mn);
-              m[n][e] = mn;
+              // f = 2^(old - new); a row that has seen no key keeps reference 0 and the next score moves it
+              const bool none = top[n][e] == -INFINITY;
+              const float mn = none ? mx : fmaxf(m[n][e], mx), f = none ? 0.f : umma::ex2(m[n][e] - mn);
+              m[n][e] = mn == -INFINITY ? 0.f : mn;
+              top[n][e] = mn + kRescaleLog2;
               l[n][e] *= f;
 #pragma unroll
               for (int gr = 0; gr < kG; ++gr) {
@@ -441,8 +442,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float mm = m[n][e & 1];
-            p[n][e] = umma::ex2(p[n][e] - (mm == -INFINITY ? 0.f : mm));
+            p[n][e] = umma::ex2(p[n][e] - m[n][e & 1]);
             l[n][e & 1] += p[n][e];
           }
         // O^T: words of keys (rows 2 t4, 2 t4 + 1, + 8) for dims 64 g + 8 gid ..
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
             for (int e = 0; e < 4; ++e) {
               w[e] = p[n][e] * sv[e >> 1][gr];
               // a key that this row does not see may hold anything, NaN scales among it
-              if (edge && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) w[e] = 0.f;
+              if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) w[e] = 0.f;
             }
             const uint32_t lo = umma::pack2_bf16(w[0], w[1]), hi = umma::pack2_bf16(w[2], w[3]);
             zc[n][gr][0] = fmaf(__uint_as_float(lo << 16), zv[0][gr], fmaf(__uint_as_float(hi << 16), zv[1][gr], zc[n][gr][0]));
@@ -478,6 +478,15 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
             for (int n = 0; n < NT; ++n) mma_bf16(o[n][gr][j], a0, a1, a2, a3, w0[n], w1[n]);
           }
         }
+      };
+      const int at0 = warp * kWarpKeys, k0 = c * kChunk + at0;
+      if (k0 + kWarpKeys <= all_see && bad == 0u) {
+#pragma unroll
+        for (int i = 0; i < kWarpKeys; i += 16) tile(std::false_type(), at0 + i);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kWarpKeys; i += 16)
+          if (k0 + i < g.keys && !((bad >> ((at0 + i) / 16)) & 1u)) tile(std::true_type(), at0 + i);
       }
       __syncwarp();
       if (lane == 0) umma::mbar_arrive(&empty[s]);
@@ -491,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
         const int r = n * 8 + t4 * 2 + e;
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-        if (gid == 0) ml[warp * kQ + r] = make_float2(m[n][e], l[n][e]);
+        if (gid == 0) ml[warp * kQ + r] = make_float2(top[n][e] - kRescaleLog2, l[n][e]);
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           float z = zc[n][gr][e];
@@ -536,9 +545,9 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
     }
     if (!whole) {
       // pieces of this pair: cut where the shares of the blocks begin
-      const int64_t i0 = ((g.pair0 + 1) * grid - 1) / share.total;
-      const int64_t i1 = ((g.pair0 + g.chunks) * grid - 1) / share.total;
-      const int pieces = (int)(i1 - i0) + 1;
+      const int i0 = (int)(((int64_t)(g.pair0 + 1) * grid - 1) / share.total);
+      const int i1 = (int)(((int64_t)(g.pair0 + g.chunks) * grid - 1) / share.total);
+      const int pieces = i1 - i0 + 1;
       __threadfence();
       asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
       if (threadIdx.x == 0)
@@ -552,7 +561,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const Args a) {
           const size_t row = row_of(r);
           float mx = -INFINITY, sum = 0.f, acc[8] = {};
           for (int x = 0; x < pieces; ++x) {
-            const int first = (int)(max(g.pair0, share_begin(share.total, grid, i0 + x)) - g.pair0);
+            const int first = max(0, share_begin(share.total, grid, i0 + x) - g.pair0);
             const size_t slot = row * a.max_splits + first;
             const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot);
             if (v.y == 0.f) continue;              // saw no key
@@ -603,6 +612,7 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
                      counters.device() == dev && max_splits * kChunk >= cap && part_o.numel() >= T * nh * max_splits * hd &&
                      part_ml.numel() >= T * nh * max_splits * 2 && counters.numel() >= T * nh,
                  "decode workspace too small for this batch");
+  LSB_INT4_CHECK(B * nkv * ((cap + kChunk - 1) / kChunk) < INT32_MAX, "more 128-key chunks than an int32 can count");
   LSB_INT4_CHECK(T * nh < INT32_MAX && nq * (nh / nkv) <= 16 * 65535, "batch exceeds int32 rows");
   const at::cuda::CUDAGuard guard(dev);
   const int rows = (int)(nq * (nh / nkv)), nt = rows > 8 ? 2 : 1, tiles = (rows + 8 * nt - 1) / (8 * nt);
@@ -618,13 +628,13 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
     const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(most, 148 * per_sm / tiles));
     launch_pdl(kern, dim3((unsigned)grid, tiles), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(), a);
   };
-#define LSB_DEC(HD, NT, PER) go(decode_int4_kernel<HD, NT>, DecLayout<HD, NT>::kBytes, PER)
+#define LSB_DEC(HD, NT) go(decode_int4_kernel<HD, NT>, DecLayout<HD, NT>::kBytes, DecLayout<HD, NT>::kBlocks)
   if (hd == 128) {
-    if (nt == 1) LSB_DEC(128, 1, 3);
-    else LSB_DEC(128, 2, 2);
+    if (nt == 1) LSB_DEC(128, 1);
+    else LSB_DEC(128, 2);
   } else {
-    if (nt == 1) LSB_DEC(64, 1, 4);
-    else LSB_DEC(64, 2, 3);
+    if (nt == 1) LSB_DEC(64, 1);
+    else LSB_DEC(64, 2);
   }
 #undef LSB_DEC
   const cudaError_t e = cudaGetLastError();
