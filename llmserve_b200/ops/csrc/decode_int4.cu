@@ -1,20 +1,24 @@
 // Decode and verify attention against 4-bit KV pages (format: int4_pages.cuh).
 //
 // The query rows of one KV head (nq new tokens x heads per KV head) are the narrow side of the tensor
-// core products and the keys and head dims the wide one, with mma.sync m16n8k16 and fp32 sums:
-//   S^T [16 keys x 8 rows]  = C_K [16 x HD] Q^T        O^T [16 dims x 8 rows] += (C_V - 8)^T [16 x 16 keys] W^T
+// core products and the keys and head dims the wide one, with mma.sync and fp32 sums:
+//   S^T [16 keys x 8 rows] = C_K [16 x HD] Q^T        O^T [16 dims x 8 rows] += (C_V - z)^T [16 x 16 keys] W^T
 // so a tile of 16 keys costs 8 rows of padding at most (16 from nine rows on).  A tcgen05 tile would
-// need 128 of them.  The operands are the codes themselves: 128 + c is a bf16 with c in its low
-// mantissa bits (one mask-or for two nibbles), and
-//   s = sum_g sk_g (sum_d q_d (128 + c_d) - (128 + zk_g) sum_d q_d)       g: groups of 64 dims
-//   o_d = sum_j w_jg (c_jd - 8) - sum_j w_jg (zv_jg - 8)                   w_jg = p_j sv_jg, rounded to bf16
-// Taking 8 off V's code before the product (exact) keeps the long sum over keys free of an offset that
-// would have to cancel; K's sum has at most HD terms and its offset leaves a score within
-// 2^-15 sum |q| sk.  The one rounding besides the output's is w, the second operand of a bf16 product.
+// need 128 of them.
 //
-// A warp's operand layout asks K for pairs of dims (d, d + 4: one 16-bit lane each of a code word) and V
-// for pairs of keys (one PRMT joins the half words of two rows, then the same mask-or): neither needs a
-// shuffle, and the order of dims or keys inside a product is free as long as both operands share it.
+// What bounds it next to memory is the integer pipe (64 lanes a clock) that turns nibbles into operands.
+//   K: a byte 0..15 read as e4m3 is c 2^-9 exactly (subnormals and the first binade are one even grid),
+//      so masking alone makes the operand: 3 instructions for 8 codes where a 16-bit form takes 7.  The
+//      query, eight significant bits, becomes two e4m3 terms after scaling the row by a power of two;
+//      values below 2^-10 of the row's largest lose what lies under 2^-17 of it.
+//      s = sum_g sk_g (sum_d q_d c_d - zk_g sum_d q_d)     g: groups of 64 dims
+//   V: 128 + c is a bf16 with c in its low mantissa bits (a mask-or for two nibbles); less 128 + zv of its
+//      key and group it is the exact c - zv.  The other operand is w_jg = p_j sv_jg in bf16, the one
+//      rounding besides the output's.  e4m3 has too few bits for w.
+//
+// A warp's operand layout asks K for 8 dims of a key (a code word as it lies) and V for pairs of keys (one
+// PRMT joins the half words of two rows): neither needs a shuffle, and the order of dims or keys inside a
+// product is free as long as both operands share it.
 //
 // One producer warp copies 128-key chunks (codes and words of K and V, a contiguous run per page) into
 // a ring with bulk copies; four consumer warps take 32 keys of every chunk and never meet until a
@@ -27,6 +31,8 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+
+#include <cuda_fp16.h>
 
 #include <type_traits>
 
@@ -79,29 +85,46 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
+// (x & mask) | bits, one instruction
+__device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t x, uint32_t m, uint32_t z) {
+  uint32_t y;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(z));
+  return y;
 }
 // nibbles s and s + 4 of a word as the bf16 pair (128 + low, 128 + high)
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int s) { return ((w >> (4 * s)) & 0x000f000fu) | 0x43004300u; }
-// the same less 136: (c - 8) exactly
-__device__ __forceinline__ uint32_t centred(uint32_t w, int s) {
-  const uint32_t x = nibbles(w, s);
-  uint32_t y;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x43084308u));
-  return y;
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, int s) { return mask_or(w >> (4 * s), 0x000f000fu, 0x43004300u); }
+// the eight nibbles of a word less z as fp16 pairs (s, s + 4): nz = -(1024 + z) twice, nz64 = -(64 + z) twice
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t nz, uint32_t nz64, uint32_t* y) {
+  const uint32_t h = w >> 8;
+  y[0] = add_f16x2(mask_or(w, 0x000f000fu, 0x64006400u), nz);
+  y[1] = fma_f16x2(mask_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, nz64);      // (1024 + 16 c) / 16
+  y[2] = add_f16x2(mask_or(h, 0x000f000fu, 0x64006400u), nz);
+  y[3] = fma_f16x2(mask_or(h, 0x00f000f0u, 0x64006400u), 0x2c002c00u, nz64);
+}
+__device__ __forceinline__ uint32_t pack2_f16(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
 }
 
 struct Args {
@@ -289,45 +312,59 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
       r += row0;
       return ((size_t)g.b * a.nq + r / group_heads) * a.nh + g.h * group_heads + r % group_heads;
     };
-    // Q^T operand: for group g and half i, dims 64 g + 16 t4 + 8 i + (s, s + 4); row gid of each 8-row tile
+    // Q^T operand: row gid of each 8-row tile as fp16 after scaling it by a power of two to a largest value
+    // in [2^14, 2^15); for group g and word i the dims 64 g + 16 t4 + 8 i + (s, s + 4)
     uint32_t qf[NT][kG][2][4];
-    float qs[NT][kG][2];                           // sum of q over a group for rows 2 t4, 2 t4 + 1
-    int limit[NT][2];                              // keys that these two rows see
+    float back[NT][2];                             // rows 2 t4, 2 t4 + 1: what a score is multiplied by
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool live = n * 8 + gid < rows;
       const uint4* src = reinterpret_cast<const uint4*>(a.q + row_of(live ? n * 8 + gid : 0) * HD);
+      uint4 v[kG][2];
+      uint32_t most = 0;                           // bit pattern of the largest magnitude
 #pragma unroll
-      for (int gr = 0; gr < kG; ++gr) {
-        float sum = 0.f;
+      for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint4 v = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          v[gr][i] = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {v[gr][i].x, v[gr][i].y, v[gr][i].z, v[gr][i].w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum += __uint_as_float(w[e] << 16) + __uint_as_float(w[e] & 0xffff0000u);
-          qf[n][gr][i][0] = __byte_perm(v.x, v.z, 0x5410);
-          qf[n][gr][i][1] = __byte_perm(v.x, v.z, 0x7632);
-          qf[n][gr][i][2] = __byte_perm(v.y, v.w, 0x5410);
-          qf[n][gr][i][3] = __byte_perm(v.y, v.w, 0x7632);
+          for (int e = 0; e < 4; ++e) most = max(most, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qs[n][gr][0] = __shfl_sync(0xffffffffu, sum, t4 * 8);
-        qs[n][gr][1] = __shfl_sync(0xffffffffu, sum, t4 * 8 + 4);
-      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // 2^k in two factors, k = 14 - exponent (subnormals count as 2^-126)
+      const int k = 14 + 127 - max(1, (int)(most >> 7)), k0 = k >> 1, k1 = k - k0;
+      const float up0 = __uint_as_float((uint32_t)(127 + k0) << 23), up1 = __uint_as_float((uint32_t)(127 + k1) << 23);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = n * 8 + t4 * 2 + e;
-        limit[n][e] = r < rows ? min(g.keys, a.lens[g.b] - a.nq + (row0 + r) / group_heads + 1) : 0;
-      }
+      for (int gr = 0; gr < kG; ++gr)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w[4] = {v[gr][i].x, v[gr][i].y, v[gr][i].z, v[gr][i].w};
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[2 * e] = __uint_as_float(w[e] << 16) * up0 * up1;
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u) * up0 * up1;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[n][gr][i][e] = pack2_f16(x[e], x[e + 4]);
+        }
+      // an infinity or NaN in the row: NaN scores
+      const float down = most >= 0x7f80u ? __uint_as_float(0x7fc00000u)
+                                         : __uint_as_float((uint32_t)(127 - k0) << 23) * a.scale_log2 *
+                                               __uint_as_float((uint32_t)(127 - k1) << 23);
+      back[n][0] = __shfl_sync(0xffffffffu, down, t4 * 8);
+      back[n][1] = __shfl_sync(0xffffffffu, down, t4 * 8 + 4);
     }
+    // keys that row r of the block sees
+    auto limit = [&](int r) { return r < rows ? min(g.keys, a.lens[g.b] - a.nq + (row0 + r) / group_heads + 1) : 0; };
     // keys below this are seen by every row of the tile
     const int all_see = min(g.keys, a.lens[g.b] - a.nq + row0 / group_heads + 1);
 
     float o[NT][kG][4][4];
     // m: the reference that exponents are taken from, top: the score that moves it (-inf: none seen yet)
-    float m[NT][2], top[NT][2], l[NT][2], zc[NT][kG][2];
+    float m[NT][2], top[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -341,8 +378,6 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
         m[n][e] = 0.f;
         top[n][e] = -INFINITY;
         l[n][e] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < kG; ++gr) zc[n][gr][e] = 0.f;
       }
     }
 
@@ -350,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
       const int s = it % L::kStages;
       ok = ok && __all_sync(0xffffffffu, wait_phase(&full[s], (it / L::kStages) & 1, abort_v, a.status, kTimeoutTmaFull));
       if (!ok) break;
-      const uint32_t st = smem_u32(smem) + s * L::kStage;
+      const uint8_t* st = smem + s * L::kStage;
       const uint32_t bad = bad_tiles[s];
       // 16 keys; edge: some row of this block does not see some of them
       auto tile = [&](auto edge, int at) {
@@ -358,60 +393,55 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
         // Row m of the tile is key (m & 8) + ((m & 7) >> 1) + 4 (m & 1): the four rows that the four lanes
         // of a group read together for V then lie in two bank halves instead of one.
         const int key_a = (gid >> 1) + 4 * (gid & 1), key_b = key_a + 8;
-        const uint32_t ka = st + (at + key_a) * (HD / 2), kb = ka + 8 * (HD / 2);
-        float sacc[NT][kG][4];
+        const uint8_t* ka = st + (at + key_a) * (HD / 2) + t4 * 8;
+        const uint8_t* kw = st + 2 * L::kCodes;
+        const uint8_t* vw = kw + L::kWords;
+        // scale words of a key: group 0 in the low half word, group 1 in the high one
+        auto words = [&](const uint8_t* w, int key) -> uint32_t {
+          if constexpr (kG == 2) return reinterpret_cast<const uint32_t*>(w)[key];
+          else return reinterpret_cast<const uint16_t*>(w)[key];
+        };
+        auto scale = [](uint32_t w, int gr) { return __uint_as_float((gr == 0 ? w << 16 : w) & 0x7ff00000u); };
+        const uint32_t kwa = words(kw, at + key_a), kwb = words(kw, at + key_b);
+        const uint32_t vwa = words(vw, at + key_a), vwb = words(vw, at + key_b);
+        float p[NT][4];                            // [key a row 0, key a row 1, key b row 0, key b row 1]
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
-          const uint2 wa = lds64(ka + gr * 32 + t4 * 8), wb = lds64(kb + gr * 32 + t4 * 8);
+          const uint2 wa = *reinterpret_cast<const uint2*>(ka + gr * 32);
+          const uint2 wb = *reinterpret_cast<const uint2*>(ka + gr * 32 + 8 * (HD / 2));
+          // -(1024 + z) of each key, twice, and -(64 + z)
+          const uint32_t za = mask_or(__byte_perm(kwa, 0, gr ? 0x3232 : 0x1010), 0x000f000fu, 0xe400e400u);
+          const uint32_t zb = mask_or(__byte_perm(kwb, 0, gr ? 0x3232 : 0x1010), 0x000f000fu, 0xe400e400u);
+          const uint32_t za64 = add_f16x2(za, 0x63806380u), zb64 = add_f16x2(zb, 0x63806380u);
+          float sacc[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sacc[n][gr][e] = 0.f;
+            for (int e = 0; e < 4; ++e) sacc[n][e] = 0.f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t xa = i ? wa.y : wa.x, xb = i ? wb.y : wb.x;
+            uint32_t ya[4], yb[4];
+            codes_f16(i ? wa.y : wa.x, za, za64, ya);
+            codes_f16(i ? wb.y : wb.x, zb, zb64, yb);
 #pragma unroll
-            for (int p = 0; p < 4; p += 2) {
-              const uint32_t a0 = nibbles(xa, p), a1 = nibbles(xb, p), a2 = nibbles(xa, p + 1), a3 = nibbles(xb, p + 1);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_bf16(sacc[n][gr], a0, a1, a2, a3, qf[n][gr][i][p], qf[n][gr][i][p + 1]);
-            }
+              for (int e = 0; e < 4; e += 2)
+                mma_f16(sacc[n], ya[e], yb[e], ya[e + 1], yb[e + 1], qf[n][gr][i][e], qf[n][gr][i][e + 1]);
           }
+          const float ska = scale(kwa, gr), skb = scale(kwb, gr);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[n][e] = fmaf(e < 2 ? ska : skb, sacc[n][e], gr == 0 ? 0.f : p[n][e]);
         }
-        // scale words of keys a and b: group 0 in the low half word, group 1 in the high one
-        const uint32_t kw = st + 2 * L::kCodes, vw = kw + L::kWords;
-        float sk[2][kG], zk[2][kG], sv[2][kG], zv[2][kG];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = at + (e ? key_b : key_a);
-          uint32_t x, y;
-          if constexpr (kG == 2) {
-            x = lds32(kw + key * 4);
-            y = lds32(vw + key * 4);
-          } else {
-            x = lds16(kw + key * 2) << 16;
-            y = lds16(vw + key * 2) << 16;
-          }
-#pragma unroll
-          for (int gr = 0; gr < kG; ++gr) {
-            const uint32_t xw = kG == 2 && gr == 0 ? x << 16 : x, yw = kG == 2 && gr == 0 ? y << 16 : y;
-            sk[e][gr] = __uint_as_float(xw & 0x7ff00000u) * a.scale_log2;
-            zk[e][gr] = __uint_as_float((xw & 0x000f0000u) | 0x43000000u);          // 128 + z
-            sv[e][gr] = __uint_as_float(yw & 0x7ff00000u);
-            zv[e][gr] = __uint_as_float((yw & 0x000f0000u) | 0x43000000u) - 136.f;  // z - 8
-          }
-        }
-        float p[NT][4];                            // [key a row 0, key a row 1, key b row 0, key b row 1]
         bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x = 0.f;
-#pragma unroll
-            for (int gr = 0; gr < kG; ++gr)
-              x = fmaf(sk[e >> 1][gr], fmaf(-zk[e >> 1][gr], qs[n][gr][e & 1], sacc[n][gr][e]), x);
-            if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) x = -INFINITY;
+            float x = p[n][e] * back[n][e & 1];
+            if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(n * 8 + t4 * 2 + (e & 1))) x = -INFINITY;
             p[n][e] = x;
             grow |= x > top[n][e & 1];
           }
@@ -432,7 +462,6 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
               l[n][e] *= f;
 #pragma unroll
               for (int gr = 0; gr < kG; ++gr) {
-                zc[n][gr][e] *= f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[n][gr][j][e] *= f, o[n][gr][j][e + 2] *= f;
               }
@@ -445,8 +474,11 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
             p[n][e] = umma::ex2(p[n][e] - m[n][e & 1]);
             l[n][e & 1] += p[n][e];
           }
-        // O^T: words of keys (rows 2 t4, 2 t4 + 1, + 8) for dims 64 g + 8 gid ..
-        const uint32_t v0 = st + L::kCodes + (at + t4) * (HD / 2) + gid * 4;
+        // O^T: words of keys (rows 2 t4, 2 t4 + 1, + 8) for dims 64 g + 8 gid ..; row 2 t4 is key t4, row
+        // 2 t4 + 1 key t4 + 4
+        const uint8_t* v0 = st + L::kCodes + (at + t4) * (HD / 2) + gid * 4;
+        const uint32_t z0 = words(vw, at + t4), z1 = words(vw, at + t4 + 4), z8 = words(vw, at + t4 + 8),
+                       z9 = words(vw, at + t4 + 12);
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           uint32_t w0[NT], w1[NT];
@@ -455,25 +487,27 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              w[e] = p[n][e] * sv[e >> 1][gr];
+              w[e] = p[n][e] * scale(e < 2 ? vwa : vwb, gr);
               // a key that this row does not see may hold anything, NaN scales among it
-              if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit[n][e & 1]) w[e] = 0.f;
+              if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(n * 8 + t4 * 2 + (e & 1))) w[e] = 0.f;
             }
             const uint32_t lo = umma::pack2_bf16(w[0], w[1]), hi = umma::pack2_bf16(w[2], w[3]);
-            zc[n][gr][0] = fmaf(__uint_as_float(lo << 16), zv[0][gr], fmaf(__uint_as_float(hi << 16), zv[1][gr], zc[n][gr][0]));
-            zc[n][gr][1] = fmaf(__uint_as_float(lo & 0xffff0000u), zv[0][gr],
-                                fmaf(__uint_as_float(hi & 0xffff0000u), zv[1][gr], zc[n][gr][1]));
             w0[n] = transpose8x8(lo);
             w1[n] = transpose8x8(hi);
           }
-          const uint32_t va = v0 + gr * 32;        // row 2 t4 is key t4, row 2 t4 + 1 key t4 + 4
-          const uint32_t x0 = lds32(va), x1 = lds32(va + 4 * (HD / 2)), x8 = lds32(va + 8 * (HD / 2)),
-                         x9 = lds32(va + 12 * (HD / 2));
+          const uint32_t x0 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32),
+                         x1 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 4 * (HD / 2)),
+                         x8 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 8 * (HD / 2)),
+                         x9 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 12 * (HD / 2));
+          // 128 + z of the two keys of each pair
+          const uint32_t z01 = mask_or(__byte_perm(z0, z1, gr ? 0x7632 : 0x5410), 0x000f000fu, 0x43004300u);
+          const uint32_t z89 = mask_or(__byte_perm(z8, z9, gr ? 0x7632 : 0x5410), 0x000f000fu, 0x43004300u);
           const uint32_t lo01 = __byte_perm(x0, x1, 0x5410), hi01 = __byte_perm(x0, x1, 0x7632);
           const uint32_t lo89 = __byte_perm(x8, x9, 0x5410), hi89 = __byte_perm(x8, x9, 0x7632);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t a0 = centred(lo01, j), a1 = centred(hi01, j), a2 = centred(lo89, j), a3 = centred(hi89, j);
+            const uint32_t a0 = sub_bf16x2(nibbles(lo01, j), z01), a1 = sub_bf16x2(nibbles(hi01, j), z01),
+                           a2 = sub_bf16x2(nibbles(lo89, j), z89), a3 = sub_bf16x2(nibbles(hi89, j), z89);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma_bf16(o[n][gr][j], a0, a1, a2, a3, w0[n], w1[n]);
           }
@@ -503,13 +537,9 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
         if (gid == 0) ml[warp * kQ + r] = make_float2(top[n][e] - kRescaleLog2, l[n][e]);
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
-          float z = zc[n][gr][e];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
           float* dst = merge + (warp * kQ + r) * L::kRow + gr * 64 + gid * 8;
-          *reinterpret_cast<float4*>(dst) = make_float4(o[n][gr][0][e] - z, o[n][gr][1][e] - z, o[n][gr][2][e] - z, o[n][gr][3][e] - z);
-          *reinterpret_cast<float4*>(dst + 4) =
-              make_float4(o[n][gr][0][e + 2] - z, o[n][gr][1][e + 2] - z, o[n][gr][2][e + 2] - z, o[n][gr][3][e + 2] - z);
+          *reinterpret_cast<float4*>(dst) = make_float4(o[n][gr][0][e], o[n][gr][1][e], o[n][gr][2][e], o[n][gr][3][e]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[n][gr][0][e + 2], o[n][gr][1][e + 2], o[n][gr][2][e + 2], o[n][gr][3][e + 2]);
         }
       }
     asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
