@@ -84,9 +84,9 @@ void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw,
 void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,
                    at::Tensor k_w, double eps, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                    at::Tensor slots, int64_t nh, at::Tensor status);
-void attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
-                    at::Tensor cu_q, int64_t nq, at::Tensor k_lens, at::Tensor tables, double scale,
-                    at::Tensor status);
+void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                            at::Tensor cu_q, at::Tensor k_lens, at::Tensor tables, double scale, int64_t max_q,
+                            at::Tensor status);
 void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                            int64_t nq, at::Tensor lens, at::Tensor tables, double scale, at::Tensor part_o,
                            at::Tensor part_ml, at::Tensor counters, int64_t max_splits, at::Tensor status);
@@ -143,7 +143,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("store_kvcache_int4", &lsb::store_kvcache_int4);
   m.def("load_kvcache_int4", &lsb::load_kvcache_int4);
   m.def("qkv_rope_int4", &lsb::qkv_rope_int4);
-  m.def("attention_int4", &lsb::attention_int4);
+  m.def("prefill_attention_int4", &lsb::prefill_attention_int4);
   m.def("decode_attention_int4", &lsb::decode_attention_int4);
   m.def("step_maps", &lsb::step_maps);
   m.def("greedy_accept", &lsb::greedy_accept);

@@ -34,6 +34,7 @@
 
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "int4_pages.cuh"
@@ -634,6 +635,7 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
   const int64_t B = lens.size(0), T = q.size(0), nh = q.size(1), nkv = kc.size(1), hd = q.size(2), bs = kc.size(2);
   LSB_INT4_CHECK(tables.size(0) >= B, "block_tables must hold one row per sequence");
   LSB_INT4_CHECK(nq >= 1 && T == B * nq, "q must hold nq rows per sequence");
+  LSB_INT4_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
   if (T == 0) return;
   const int64_t cap = tables.size(1) * bs;
   LSB_INT4_CHECK(part_o.scalar_type() == at::kFloat && part_ml.scalar_type() == at::kFloat &&

@@ -1,0 +1,489 @@
+// Varlen causal attention of query chunks against 4-bit KV pages (format: int4_pages.cuh) on the
+// 5th-generation tensor cores: S = Q K^T and O += P V as tcgen05.mma with fp32 accumulators in TMEM.
+//
+// The query rows of one KV head are (query, head of its group) pairs, query-major; a block computes two
+// 128-row tiles ("A", "B") of them against the same 128-key tiles, so a key is dequantised once for
+// 256 rows whatever the group size, and short chunks still fill the tile.
+//   warps 0..3 / 4..7 : softmax of tile A / B, a thread per row.  Two passes over the row's 128 scores in
+//                    TMEM (maximum; exponentials), 32 columns at a time, so nothing waits on 128
+//                    registers.  P replaces S in TMEM as bf16 (columns 16 c .. of chunk c: behind what
+//                    has been read) and is the PV product's A operand from there: it never passes
+//                    through shared memory.  The reference maximum moves only when a score passes it by
+//                    2^8; O is then rescaled in TMEM (its last PV is done: S of this tile was issued after).
+//   warps 8..11    : dequantise K and V tiles into two-stage rings in the 128B-swizzled layouts the
+//                    products read (K K-major, V MN-major).  A page row's 16 bytes are 32 dims; a code
+//                    pair is (nibble s, nibble s + 4) of a word, so every 8 dims stand in the order
+//                    0 4 1 5 2 6 3 7: Q's rows are written in that order too, and O's columns are put
+//                    back at the end.  128 + c is a bf16 with c in its mantissa; less 128 + z, times the
+//                    scale, both exact.  Eight lanes take eight keys of the same chunk: no bank conflict.
+//                    The next tile's codes and words are loaded before this one is written.
+//   warp 12, lane 0: MMA issuer: PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): while one tile's softmax works the
+//                    other tile's products run.
+// Keys past the block's last visible one, or in a block outside the pool (recorded), are zeros in both
+// tiles and masked in S.  A V group that holds NaN is zeroed too and flagged: only the rows that see the
+// key return NaN for that group.  Every wait is bounded; a timeout records an error and every role ends.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <cmath>
+
+#include "int4_pages.cuh"
+#include "umma.cuh"
+
+namespace lsb {
+
+int* status_ptr(const at::Tensor& status);
+
+namespace {
+
+using namespace int4;
+using namespace umma;
+
+constexpr int kBQ = 128;                  // rows of a tile (UMMA M)
+constexpr int kBK = 128;                  // keys of a tile
+constexpr int kThreads = 13 * 32;
+constexpr float kRescaleLog2 = 8.f;
+
+template <int HD>
+struct PfLayout {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kHalf = 128 * 128;                 // 128 rows of 128 bytes
+  static constexpr int kTile = kHalves * kHalf;
+  static constexpr int kKOff = 2 * kTile;                 // after the two Q tiles
+  static constexpr int kVOff = kKOff + 2 * kTile;
+  static constexpr int kBarOff = kVOff + 2 * kTile;
+  static constexpr int kBytes = kBarOff + 512 + 1024;     // barriers and flags, alignment slack
+};
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+
+// What softmax has to know of a 128-key tile beyond its position: per dequantising warp (32 keys) the
+// keys that are not there and those whose V group 0 / 1 is NaN; `any` is their union, read first.
+struct TileFlags {
+  uint32_t any[4], gone[4], nan0[4], nan1[4];
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
+    bf16* __restrict__ out, const bf16* __restrict__ q, Pages kp, Pages vp, const int* __restrict__ cu_q,
+    const int* __restrict__ k_lens, const int* __restrict__ tables, int width, int B, int T, float scale_log2, int nh,
+    int nkv, int bs, int nblk, int pairs, int* __restrict__ status) {
+  using L = PfLayout<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
+           *s_full = bars + 9, *p_full = bars + 11, *drain = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  TileFlags* flags = reinterpret_cast<TileFlags*>(smem + L::kBarOff + 128);    // four tiles' worth
+  __shared__ int abort_flag;
+  volatile int* abort_v = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_trigger();
+  pdl_wait();
+  // the blocks with most keys first: blockIdx.y enumerates (pair of tiles from the last, sequence)
+  const int pair = pairs - 1 - (int)blockIdx.y / B, seq = (int)blockIdx.y % B, kvh = blockIdx.x;
+  const int G = nh / nkv, per_tile = kBQ / G;              // queries of a tile
+  const int q0 = max(0, min(T, cu_q[seq])), q_len = min(cu_q[seq + 1], T) - q0;
+  const int first = pair * 2 * per_tile;
+  if (first >= q_len) return;
+  const int k_cap = max(0, min(k_lens[seq], (int)min((int64_t)width * bs, (int64_t)INT32_MAX - kBK)));
+  const int shift = k_lens[seq] - q_len;                   // absolute position of query 0
+  int kend_t[2], nt[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int a = first + t * per_tile, last = min(q_len, a + per_tile) - 1;
+    kend_t[t] = a < q_len ? max(0, min(k_cap, shift + last + 1)) : 0;
+    nt[t] = (kend_t[t] + kBK - 1) / kBK;
+  }
+  const int kend = max(kend_t[0], kend_t[1]), ntiles = max(nt[0], nt[1]);
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(q_full, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;                        // S (then P) of tile t at 128 t, O at 256 + 128 t
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------- dequantisation ----------------
+    constexpr int kCpk = HD / 32;                          // 16-byte chunks of a key
+    constexpr int kKps = 32 / kCpk;                        // keys of a step
+    constexpr int kSteps = 32 / kKps;
+    const int w = warp - 8;
+    const int chunk = (lane >> 3) % kCpk, half = chunk >> 1;
+    const int key0 = (lane & 7) + 8 * ((lane >> 3) / kCpk);          // within a step
+    const int* table = tables + (int64_t)seq * width;
+    uint4 kc[kSteps], vc[kSteps];
+    uint32_t kw[kSteps], vw[kSteps];
+    // rows of this warp's two 16-key tiles of key tile j (lanes 0, 1), in units of 16; -1: nothing there
+    auto find_rows = [&](int j) {
+      const int k = j * kBK + w * 32 + (lane & 1) * 16;
+      if (k >= kend) return -1;
+      const int page = k / bs, blk = table[page];
+      if (blk < 0 || blk >= nblk) {
+        if (lane < 2) record_error(status, kBadIndex);
+        return -2;
+      }
+      return (int)((((int64_t)blk * nkv + kvh) * bs + (k - page * bs)) / 16);
+    };
+    auto row_of = [&](int rows, int i, bool& ok, int j) {
+      const int key = i * kKps + key0;
+      const int r = __shfl_sync(0xffffffffu, rows, key >> 4);
+      ok = r >= 0 && j * kBK + w * 32 + key < kend;
+      return (int64_t)(ok ? r : 0) * 16 + (key & 15);
+    };
+    auto load = [&](int rows, int j, uint4* kc, uint4* vc, uint32_t* kw, uint32_t* vw) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        bool ok;
+        const int64_t row = row_of(rows, i, ok, j);
+        kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
+        kw[i] = vw[i] = 0;                                 // scale 0: the key reads as zeros
+        if (ok) {
+          kc[i] = __ldg(reinterpret_cast<const uint4*>(kp.codes + row * (HD / 2)) + chunk);
+          vc[i] = __ldg(reinterpret_cast<const uint4*>(vp.codes + row * (HD / 2)) + chunk);
+          kw[i] = (uint16_t)__ldg(kp.words + row * L::kHalves + half);
+          vw[i] = (uint16_t)__ldg(vp.words + row * L::kHalves + half);
+        }
+      }
+    };
+    auto put = [&](uint8_t* tile, const uint4* c, const uint32_t* sw) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int key = w * 32 + i * kKps + key0;
+        const uint32_t dup = __byte_perm(sw[i], 0, 0x1010);
+        const uint32_t s2 = dup & 0x7ff07ff0u, z2 = mask_or(dup, 0x000f000fu, 0x43004300u);
+        uint8_t* row = tile + half * L::kHalf + key * 128;
+        const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          uint32_t y[4];
+#pragma unroll
+          for (int s = 0; s < 4; ++s) y[s] = mul2(sub2(mask_or(words[p] >> (4 * s), 0x000f000fu, 0x43004300u), z2), s2);
+          const int c16 = (chunk & 1) * 4 + p;
+          *reinterpret_cast<uint4*>(row + ((c16 ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+    };
+    bool ok = true;
+    int rows = ntiles > 0 ? find_rows(0) : -1;
+    if (ntiles > 0) load(rows, 0, kc, vc, kw, vw);
+    int next = ntiles > 1 ? find_rows(1) : -1;
+    for (int j = 0; j < ntiles; ++j) {
+      const int s = j & 1, u = j >> 1;
+      // flags of this tile (a tile four before it is out of use: its softmax ended before S of j - 2 began)
+      bool odd = rows == -2 && lane < 2;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) odd |= (vw[i] & 0x7f80u) == 0x7f80u;
+      uint32_t any = 0;
+      if (__any_sync(0xffffffffu, odd)) {
+        uint32_t gone = 0, nan[2] = {0, 0};
+        if (__shfl_sync(0xffffffffu, rows, 0) == -2) gone |= 0xffffu;
+        if (__shfl_sync(0xffffffffu, rows, 1) == -2) gone |= 0xffff0000u;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const bool bad = (vw[i] & 0x7f80u) == 0x7f80u;
+          if (bad) vw[i] = 0;                              // zeros, and a flag for those who see it
+          const uint32_t at = bad ? 1u << (i * kKps + key0) : 0u;
+          nan[0] |= __reduce_or_sync(0xffffffffu, half == 0 ? at : 0u);
+          nan[1] |= __reduce_or_sync(0xffffffffu, half == 1 ? at : 0u);
+        }
+        any = gone | nan[0] | nan[1];
+        if (lane == 0) {
+          flags[j & 3].gone[w] = gone;
+          flags[j & 3].nan0[w] = nan[0];
+          flags[j & 3].nan1[w] = nan[1];
+        }
+      }
+      if (lane == 0) flags[j & 3].any[w] = any;
+      uint4 kc1[kSteps], vc1[kSteps];
+      uint32_t kw1[kSteps], vw1[kSteps];
+      if (j + 1 < ntiles) load(next, j + 1, kc1, vc1, kw1, vw1);
+      const int after = j + 2 < ntiles ? find_rows(j + 2) : -1;
+      if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&k_empty[s], (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+      if (!ok) break;
+      put(smem + L::kKOff + s * L::kTile, kc, kw);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[s]);
+      if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&v_empty[s], (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+      if (!ok) break;
+      put(smem + L::kVOff + s * L::kTile, vc, vw);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_full[s]);
+      if (j + 1 < ntiles) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) kc[i] = kc1[i], vc[i] = vc1[i], kw[i] = kw1[i], vw[i] = vw1[i];
+      }
+      rows = next;
+      next = after;
+    }
+  } else if (warp == 12) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0 && ntiles > 0) {
+      constexpr uint32_t id_s = idesc_f16(kBQ, kBK, false), id_pv = idesc_f16(kBQ, HD, true);
+      const uint32_t qa = smem_u32(smem);
+      bool ok = wait_phase(q_full, 0, abort_v, status, kTimeoutTmaFull);
+      auto issue_s = [&](int t, int j) {
+        const int s = j & 1;
+        if (!wait_phase(&k_full[s], (j >> 1) & 1, abort_v, status, kTimeoutTmaFull)) return false;
+        fence_after();
+        const uint32_t ka = smem_u32(smem + L::kKOff + s * L::kTile);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          mma(tmem + t * 128, desc_kmajor(qa + t * L::kTile + (k / 4) * L::kHalf + (k % 4) * 32),
+              desc_kmajor(ka + (k / 4) * L::kHalf + (k % 4) * 32), id_s, k != 0);
+        commit(&s_full[t]);
+        if (t == 1 || j >= nt[1]) commit(&k_empty[s]);     // the last S that reads this K tile
+        return true;
+      };
+      auto issue_pv = [&](int t, int j) {
+        const int s = j & 1;
+        if (!wait_phase(&p_full[t], j & 1, abort_v, status, kTimeoutAccum)) return false;
+        if (!wait_phase(&v_full[s], (j >> 1) & 1, abort_v, status, kTimeoutTmaFull)) return false;
+        fence_after();
+        const uint32_t va = smem_u32(smem + L::kVOff + s * L::kTile);
+#pragma unroll
+        for (int k = 0; k < kBK / 16; ++k)
+          mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, desc_mnmajor(va + k * 16 * 128, L::kHalf), id_pv, (j | k) != 0);
+        if (t == 1 || j >= nt[1]) commit(&v_empty[s]);
+        return true;
+      };
+      for (int t = 0; ok && t < 2; ++t)
+        if (nt[t] > 0) ok = issue_s(t, 0);
+      for (int j = 0; ok && j < ntiles; ++j)
+        for (int t = 0; ok && t < 2; ++t) {
+          if (j < nt[t]) ok = issue_pv(t, j);
+          if (ok && j + 1 < nt[t]) ok = issue_s(t, j + 1);
+          else if (ok && j + 1 == nt[t]) commit(&s_full[t]);        // one more phase: O is complete
+        }
+      commit(drain);
+      mbar_wait(drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax ----------------
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int qi = first + t * per_tile + r / G, head = kvh * G + r % G;
+    const bool live = r < per_tile * G && qi < q_len;
+    const size_t row = (size_t)(q0 + (live ? qi : 0)) * nh + head;
+    // Q row into the tile, 8 dims at a time in the order 0 4 1 5 2 6 3 7; rows without a query are zeros
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(q + row * HD);
+      uint8_t* dst = smem + t * L::kTile + r * 128;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = live ? src[c] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + (c / 8) * L::kHalf + (((c % 8) ^ (r & 7)) << 4)) =
+            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                       __byte_perm(v.y, v.w, 0x7632));
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    // keys this row sees; rows without a query take whatever comes (their result is dropped)
+    const int limit = live ? max(0, min(k_cap, shift + qi + 1)) : INT32_MAX;
+    const int warp_limit = __reduce_min_sync(0xffffffffu, limit);
+    const uint32_t base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tmem_s = tmem + t * 128 + base, tmem_o = tmem + 256 + t * 128 + base;
+    float m_used = -INFINITY, l = 0.f;
+    bool nan0 = false, nan1 = false, ok = true;
+    for (int j = 0; j < nt[t]; ++j) {
+      ok = __all_sync(0xffffffffu, wait_phase(&s_full[t], j & 1, abort_v, status, kTimeoutAccum));
+      if (!ok) break;
+      fence_after();
+      const int k0 = j * kBK;
+      const TileFlags& f = flags[j & 3];
+      const uint4 any = *reinterpret_cast<const uint4*>(f.any);
+      const bool flagged = (any.x | any.y | any.z | any.w) != 0u;
+      const bool inside = !flagged && k0 + kBK <= warp_limit;
+      // keys of chunk c that this row does not see, as a bit mask
+      auto hidden = [&](int c) {
+        const int n = limit - k0 - c * 32;
+        return (n >= 32 ? 0u : n <= 0 ? 0xffffffffu : ~0u << n) | (flagged && ((const volatile uint32_t*)f.any)[c] ? ((const volatile uint32_t*)f.gone)[c] : 0u);
+      };
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32];
+        tmem_ld16(tmem_s + c * 32, x);
+        tmem_ld16(tmem_s + c * 32 + 16, x + 16);
+        tmem_wait_ld();
+        if (!inside) {
+          const uint32_t h = hidden(c);
+          if (flagged && ((const volatile uint32_t*)f.any)[c]) {
+            nan0 |= (((const volatile uint32_t*)f.nan0)[c] & ~h) != 0u;
+            nan1 |= (((const volatile uint32_t*)f.nan1)[c] & ~h) != 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (h >> e & 1u) x[e] = 0xff800000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(x[e]));
+      }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+      float alpha = 1.f;
+      if (mx > m_used + kRescaleLog2) {
+        alpha = m_used == -INFINITY ? 0.f : ex2(m_used - mx);
+        m_used = mx;
+        l *= alpha;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(tmem_o + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st16(tmem_o + c, o);
+        }
+      }
+      const float neg_m = m_used == -INFINITY ? 0.f : -m_used;      // a row that sees nothing: all P = 0
+      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t x[32], p[16];
+        tmem_ld16(tmem_s + c * 32, x);
+        tmem_ld16(tmem_s + c * 32 + 16, x + 16);
+        tmem_wait_ld();
+        if (!inside) {
+          const uint32_t h = hidden(c);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (h >> e & 1u) x[e] = 0xff800000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float a = ex2(fmaf(__uint_as_float(x[e]), scale_log2, neg_m));
+          const float b = ex2(fmaf(__uint_as_float(x[e + 1]), scale_log2, neg_m));
+          sum4[e & 2] += a;
+          sum4[(e & 2) + 1] += b;
+          p[e / 2] = pack2_bf16(a, b);
+        }
+        tmem_st16(tmem_s + c * 16, p);
+      }
+      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+      tmem_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    // O / l, columns back in order
+    const bool done = ok && nt[t] > 0 &&
+                      __all_sync(0xffffffffu, wait_phase(&s_full[t], nt[t] & 1, abort_v, status, kTimeoutAccum));
+    fence_after();
+    uint4* dst = reinterpret_cast<uint4*>(out + row * HD);
+    if (done) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < HD; c += 16) {
+        const float i = (c < 64 ? nan0 : nan1) ? __uint_as_float(0x7fc00000u) : inv;
+        uint32_t o[16];
+        tmem_ld16(tmem_o + c, o);
+        tmem_wait_ld();
+        if (live)
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            auto v = [&](int d) { return __uint_as_float(o[e + d]) * i; };      // column d holds dim (0 4 1 5 2 6 3 7)[d]
+            dst[(c + e) / 8] = make_uint4(pack2_bf16(v(0), v(2)), pack2_bf16(v(4), v(6)), pack2_bf16(v(1), v(3)),
+                                          pack2_bf16(v(5), v(7)));
+          }
+      }
+    } else if (live && nt[t] == 0) {
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+}  // namespace
+
+void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                            at::Tensor cu_q, at::Tensor k_lens, at::Tensor tables, double scale, int64_t max_q,
+                            at::Tensor status) {
+  const at::Device dev = q.device();
+  check_page_pair(kc, kw, vc, vw, dev);
+  LSB_INT4_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
+                     reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+                 "q must be contiguous, 16-byte aligned bfloat16 [rows, heads, head_dim]");
+  const int64_t T = q.size(0), nh = q.size(1), hd = q.size(2), nkv = kc.size(1), bs = kc.size(2);
+  LSB_INT4_CHECK(hd == kc.size(3) * 2 && nh >= 1 && nh % nkv == 0, "query heads do not match the pages");
+  LSB_INT4_CHECK(nh / nkv <= kBQ, "more than 128 query heads per KV head");
+  LSB_INT4_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.is_contiguous() &&
+                     out.device() == dev, "bad output");
+  check_int32(k_lens, "sequence lengths", 1, dev);
+  check_int32(tables, "block_tables", 2, dev);
+  check_int32(cu_q, "cu_seqlens_q", 1, dev);
+  const int64_t B = k_lens.size(0);
+  LSB_INT4_CHECK(tables.size(0) >= B, "block_tables must hold one row per sequence");
+  LSB_INT4_CHECK(cu_q.size(0) == B + 1, "cu_seqlens_q must hold one entry more than there are sequences");
+  LSB_INT4_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
+  LSB_INT4_CHECK(kc.numel() / (hd / 2) / 16 < INT32_MAX && T < INT32_MAX, "pages exceed int32 rows of 16 keys");
+  if (T == 0 || B == 0 || max_q <= 0) return;
+  const at::cuda::CUDAGuard guard(dev);
+  const int64_t per = 2 * (kBQ / (nh / nkv)), pairs = (std::min(max_q, T) + per - 1) / per;
+  LSB_INT4_CHECK(pairs * B < 65536, "too many query tiles for one launch");
+  auto go = [&](auto kern, int smem) {
+    ensure_dynamic_smem((const void*)kern, smem);
+    launch_pdl(kern, dim3((unsigned)nkv, (unsigned)(pairs * B)), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(),
+               (bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), Pages{kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
+               Pages{vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, (const int*)cu_q.data_ptr<int>(),
+               (const int*)k_lens.data_ptr<int>(), (const int*)tables.data_ptr<int>(), (int)tables.size(1), (int)B, (int)T,
+               (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs, (int)kc.size(0), (int)pairs,
+               status_ptr(status));
+  };
+  if (hd == 128) go(prefill_int4_kernel<128>, PfLayout<128>::kBytes);
+  else go(prefill_int4_kernel<64>, PfLayout<64>::kBytes);
+  const cudaError_t e = cudaGetLastError();
+  LSB_INT4_CHECK(e == cudaSuccess, std::string("prefill_attention_int4 launch failed: ") + cudaGetErrorString(e));
+}
+
+}  // namespace lsb

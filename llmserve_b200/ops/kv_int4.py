@@ -229,11 +229,12 @@ def decode_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table
 def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens_q, seqlens_k, block_tables, scale,
                            max_seqlen_q: int):
     """Varlen causal attention of packed query rows ``[T, nh, hd]``; row ``j`` of a chunk of ``q_len``
-    sees keys ``< seqlens_k - q_len + j + 1``.  Rows behind the last sequence are left unwritten."""
+    sees keys ``< seqlens_k - q_len + j + 1``.  ``max_seqlen_q`` is at least the longest chunk (rows past
+    it, like rows behind the last sequence, are left unwritten)."""
     if not q.is_cuda:
         _check_pages(k_pages, v_pages)
         return attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_tables, scale)
     out = torch.empty_like(q)
-    C().attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, cu_seqlens_q, 0,
-                       seqlens_k, block_tables, scale, status(q.device))
+    C().prefill_attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words,
+                               cu_seqlens_q, seqlens_k, block_tables, scale, max_seqlen_q, status(q.device))
     return out
