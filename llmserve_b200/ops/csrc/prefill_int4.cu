@@ -61,6 +61,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
 }
+// 32 lanes x 32 columns of fp32 (no wait)
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
 __device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
   uint32_t y;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
@@ -238,18 +249,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
       uint32_t kw1[kSteps], vw1[kSteps];
       if (j + 1 < ntiles) load(next, j + 1, kc1, vc1, kw1, vw1);
       const int after = j + 2 < ntiles ? find_rows(j + 2) : -1;
-      if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&k_empty[s], (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {                     // K, then V: one copy of the code for the instruction cache
+        if (u >= 1)
+          ok = __all_sync(0xffffffffu, wait_phase((kv ? v_empty : k_empty) + s, (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+        if (!ok) break;
+        put(smem + (kv ? L::kVOff : L::kKOff) + s * L::kTile, kc, kw);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive((kv ? v_full : k_full) + s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) kc[i] = vc[i], kw[i] = vw[i];
+      }
       if (!ok) break;
-      put(smem + L::kKOff + s * L::kTile, kc, kw);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[s]);
-      if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&v_empty[s], (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
-      if (!ok) break;
-      put(smem + L::kVOff + s * L::kTile, vc, vw);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[s]);
       if (j + 1 < ntiles) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) kc[i] = kc1[i], vc[i] = vc1[i], kw[i] = kw1[i], vw[i] = vw1[i];
@@ -343,11 +355,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         return (n >= 32 ? 0u : n <= 0 ? 0xffffffffu : ~0u << n) | (flagged && ((const volatile uint32_t*)f.any)[c] ? ((const volatile uint32_t*)f.gone)[c] : 0u);
       };
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t x[32];
-        tmem_ld16(tmem_s + c * 32, x);
-        tmem_ld16(tmem_s + c * 32 + 16, x + 16);
+        tmem_ld32(tmem_s + c * 32, x);
         tmem_wait_ld();
         if (!inside) {
           const uint32_t h = hidden(c);
@@ -382,11 +393,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
       }
       const float neg_m = m_used == -INFINITY ? 0.f : -m_used;      // a row that sees nothing: all P = 0
       float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t x[32], p[16];
-        tmem_ld16(tmem_s + c * 32, x);
-        tmem_ld16(tmem_s + c * 32 + 16, x + 16);
+        tmem_ld32(tmem_s + c * 32, x);
         tmem_wait_ld();
         if (!inside) {
           const uint32_t h = hidden(c);
