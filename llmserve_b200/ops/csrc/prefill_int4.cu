@@ -10,13 +10,14 @@
 //                    has been read) and is the PV product's A operand from there: it never passes
 //                    through shared memory.  The reference maximum moves only when a score passes it by
 //                    2^8; O is then rescaled in TMEM (its last PV is done: S of this tile was issued after).
-//   warps 8..11    : dequantise K and V tiles into two-stage rings in the 128B-swizzled layouts the
-//                    products read (K K-major, V MN-major).  A page row's 16 bytes are 32 dims; a code
-//                    pair is (nibble s, nibble s + 4) of a word, so every 8 dims stand in the order
-//                    0 4 1 5 2 6 3 7: Q's rows are written in that order too, and O's columns are put
-//                    back at the end.  128 + c is a bf16 with c in its mantissa; less 128 + z, times the
-//                    scale, both exact.  Eight lanes take eight keys of the same chunk: no bank conflict.
-//                    The next tile's codes and words are loaded before this one is written.
+//   warp 13        : copies the codes and words of K and V tiles (a run per page, bulk copies) into a ring of
+//                    three entries, K and V by turns.
+//   warps 8..11    : dequantise an entry into the two-stage rings of the 128B-swizzled tiles the products
+//                    read (K K-major, V MN-major).  A code pair is (nibble s, nibble s + 4) of a word, so
+//                    every 8 dims stand in the order 0 4 1 5 2 6 3 7: Q's rows are written in that order
+//                    too, and O's columns are put back at the end.  128 + c is a bf16 with c in its
+//                    mantissa; less 128 + z, times the scale, both exact.  Lanes of the upper group take
+//                    the halves of their 16 bytes the other way round: no bank is hit twice in a store.
 //   warp 12, lane 0: MMA issuer: PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): while one tile's softmax works the
 //                    other tile's products run.
 // Keys past the block's last visible one, or in a block outside the pool (recorded), are zeros in both
@@ -42,7 +43,8 @@ using namespace umma;
 
 constexpr int kBQ = 128;                  // rows of a tile (UMMA M)
 constexpr int kBK = 128;                  // keys of a tile
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 14 * 32;
+constexpr int kEntries = 3;               // ring of packed tiles
 constexpr float kRescaleLog2 = 8.f;
 
 template <int HD>
@@ -52,7 +54,10 @@ struct PfLayout {
   static constexpr int kTile = kHalves * kHalf;
   static constexpr int kKOff = 2 * kTile;                 // after the two Q tiles
   static constexpr int kVOff = kKOff + 2 * kTile;
-  static constexpr int kBarOff = kVOff + 2 * kTile;
+  static constexpr int kRawOff = kVOff + 2 * kTile;        // packed tiles: codes, then words
+  static constexpr int kRawCodes = kBK * HD / 2;
+  static constexpr int kRaw = kRawCodes + kBK * kHalves * 2;
+  static constexpr int kBarOff = kRawOff + kEntries * kRaw;
   static constexpr int kBytes = kBarOff + 512 + 1024;     // barriers and flags, alignment slack
 };
 
@@ -72,6 +77,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
   uint32_t y;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
@@ -88,10 +98,10 @@ __device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t 
   return y;
 }
 
-// What softmax has to know of a 128-key tile beyond its position: per dequantising warp (32 keys) the
-// keys that are not there and those whose V group 0 / 1 is NaN; `any` is their union, read first.
+// What softmax has to know of a 128-key tile beyond its position, a bit per key: keys that are not there
+// (known when K is), and those whose V group 0 / 1 is NaN (known when V is).
 struct TileFlags {
-  uint32_t any[4], gone[4], nan0[4], nan1[4];
+  uint32_t gone[4], nan0[4], nan1[4];
 };
 
 template <int HD>
@@ -104,9 +114,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-           *s_full = bars + 9, *p_full = bars + 11, *drain = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
-  TileFlags* flags = reinterpret_cast<TileFlags*>(smem + L::kBarOff + 128);    // four tiles' worth
+           *s_full = bars + 9, *p_full = bars + 11, *drain = bars + 13, *raw_full = bars + 14,
+           *raw_empty = raw_full + kEntries;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + kEntries);
+  volatile uint32_t* raw_gone = tmem_slot + 1;             // 16-key tiles of an entry that are not there
+  TileFlags* flags = reinterpret_cast<TileFlags*>(smem + L::kBarOff + 256);    // four tiles' worth
   __shared__ int abort_flag;
   volatile int* abort_v = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -141,6 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
     }
+    for (int e = 0; e < kEntries; ++e) {
+      mbar_init(&raw_full[e], 1);
+      mbar_init(&raw_empty[e], 4);
+    }
     mbar_init(drain, 1);
     fence_barrier_init();
   }
@@ -157,133 +173,126 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     // ---------------- dequantisation ----------------
     constexpr int kCpk = HD / 32;                          // 16-byte chunks of a key
     constexpr int kKps = 32 / kCpk;                        // keys of a step
-    constexpr int kSteps = 32 / kKps;
     const int w = warp - 8;
-    const int chunk = (lane >> 3) % kCpk, half = chunk >> 1;
-    const int key0 = (lane & 7) + 8 * ((lane >> 3) / kCpk);          // within a step
-    const int* table = tables + (int64_t)seq * width;
-    uint4 kc[kSteps], vc[kSteps];
-    uint32_t kw[kSteps], vw[kSteps];
-    // rows of this warp's two 16-key tiles of key tile j (lanes 0, 1), in units of 16; -1: nothing there
-    auto find_rows = [&](int j) {
-      const int k = j * kBK + w * 32 + (lane & 1) * 16;
-      if (k >= kend) return -1;
-      const int page = k / bs, blk = table[page];
-      if (blk < 0 || blk >= nblk) {
-        if (lane < 2) record_error(status, kBadIndex);
-        return -2;
-      }
-      return (int)((((int64_t)blk * nkv + kvh) * bs + (k - page * bs)) / 16);
-    };
-    auto row_of = [&](int rows, int i, bool& ok, int j) {
-      const int key = i * kKps + key0;
-      const int r = __shfl_sync(0xffffffffu, rows, key >> 4);
-      ok = r >= 0 && j * kBK + w * 32 + key < kend;
-      return (int64_t)(ok ? r : 0) * 16 + (key & 15);
-    };
-    auto load = [&](int rows, int j, uint4* kc, uint4* vc, uint32_t* kw, uint32_t* vw) {
+    const int chunk = lane % kCpk, half = chunk >> 1, key0 = w * 32 + lane / kCpk;
+    // words 2 h and 2 h + 1 of the chunk first (h = half), then the other two; their places in the tile
+    const uint32_t src0 = key0 * (HD / 2) + chunk * 16 + half * 8;
+    uint32_t place[4];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        bool ok;
-        const int64_t row = row_of(rows, i, ok, j);
-        kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
-        kw[i] = vw[i] = 0;                                 // scale 0: the key reads as zeros
-        if (ok) {
-          kc[i] = __ldg(reinterpret_cast<const uint4*>(kp.codes + row * (HD / 2)) + chunk);
-          vc[i] = __ldg(reinterpret_cast<const uint4*>(vp.codes + row * (HD / 2)) + chunk);
-          kw[i] = (uint16_t)__ldg(kp.words + row * L::kHalves + half);
-          vw[i] = (uint16_t)__ldg(vp.words + row * L::kHalves + half);
+    for (int p = 0; p < 4; ++p)
+      place[p] = half * L::kHalf + key0 * 128 + ((((chunk & 1) * 4 + (p ^ (half * 2))) ^ (key0 & 7)) << 4);
+    bool ok = true;
+#pragma unroll 1
+    for (int e = 0; e < 2 * ntiles; ++e) {                 // K of tile 0, V of tile 0, K of tile 1, ..
+      const int j = e >> 1, kv = e & 1, s = j & 1, u = j >> 1, re = e % kEntries;
+      ok = __all_sync(0xffffffffu, wait_phase(&raw_full[re], (e / kEntries) & 1, abort_v, status, kTimeoutTmaFull));
+      if (ok && u >= 1)
+        ok = __all_sync(0xffffffffu, wait_phase((kv ? v_empty : k_empty) + s, (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+      if (!ok) break;
+      const uint8_t* raw = smem + L::kRawOff + re * L::kRaw;
+      const uint16_t* words = reinterpret_cast<const uint16_t*>(raw + L::kRawCodes);
+      uint8_t* tile = smem + (kv ? L::kVOff : L::kKOff) + s * L::kTile;
+      // keys of this warp that read as zeros: past the last one, or in a block that is not there
+      const uint32_t gone16 = raw_gone[re] >> (w * 2) & 3u;
+      const uint32_t gone = (gone16 & 1u ? 0xffffu : 0u) | (gone16 & 2u ? 0xffff0000u : 0u);
+      const int left = kend - j * kBK - w * 32;
+      const uint32_t zero = gone | (left >= 32 ? 0u : left <= 0 ? 0xffffffffu : ~0u << left);
+      uint32_t nan[2] = {0, 0};
+#pragma unroll 1
+      for (int i = 0; i < 32 / kKps; ++i) {
+        const int in_warp = lane / kCpk + i * kKps;
+        const uint2 c0 = *reinterpret_cast<const uint2*>(raw + src0 + i * kKps * (HD / 2));
+        const uint2 c1 = *reinterpret_cast<const uint2*>(raw + (src0 ^ 8u) + i * kKps * (HD / 2));
+        uint32_t sw = words[(key0 + i * kKps) * L::kHalves + half];
+        if (zero >> in_warp & 1u) sw = 0;                  // scale 0
+        const bool bad = kv && (sw & 0x7f80u) == 0x7f80u;
+        if (__any_sync(0xffffffffu, bad)) {                // zeros, and a flag for the rows that see the key
+          const uint32_t bit = bad ? 1u << in_warp : 0u;
+          nan[0] |= __reduce_or_sync(0xffffffffu, half == 0 ? bit : 0u);
+          nan[1] |= __reduce_or_sync(0xffffffffu, half == 1 ? bit : 0u);
+          if (bad) sw = 0;
         }
-      }
-    };
-    auto put = [&](uint8_t* tile, const uint4* c, const uint32_t* sw) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int key = w * 32 + i * kKps + key0;
-        const uint32_t dup = __byte_perm(sw[i], 0, 0x1010);
+        const uint32_t dup = __byte_perm(sw, 0, 0x1010);
         const uint32_t s2 = dup & 0x7ff07ff0u, z2 = mask_or(dup, 0x000f000fu, 0x43004300u);
-        uint8_t* row = tile + half * L::kHalf + key * 128;
-        const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+        const uint32_t c[4] = {c0.x, c0.y, c1.x, c1.y};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           uint32_t y[4];
 #pragma unroll
-          for (int s = 0; s < 4; ++s) y[s] = mul2(sub2(mask_or(words[p] >> (4 * s), 0x000f000fu, 0x43004300u), z2), s2);
-          const int c16 = (chunk & 1) * 4 + p;
-          *reinterpret_cast<uint4*>(row + ((c16 ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+          for (int n = 0; n < 4; ++n) y[n] = mul2(sub2(mask_or(c[p] >> (4 * n), 0x000f000fu, 0x43004300u), z2), s2);
+          *reinterpret_cast<uint4*>(tile + place[p] + i * kKps * 128) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       }
-    };
-    bool ok = true;
-    int rows = ntiles > 0 ? find_rows(0) : -1;
-    if (ntiles > 0) load(rows, 0, kc, vc, kw, vw);
-    int next = ntiles > 1 ? find_rows(1) : -1;
-    for (int j = 0; j < ntiles; ++j) {
-      const int s = j & 1, u = j >> 1;
-      // flags of this tile (a tile four before it is out of use: its softmax ended before S of j - 2 began)
-      bool odd = rows == -2 && lane < 2;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) odd |= (vw[i] & 0x7f80u) == 0x7f80u;
-      uint32_t any = 0;
-      if (__any_sync(0xffffffffu, odd)) {
-        uint32_t gone = 0, nan[2] = {0, 0};
-        if (__shfl_sync(0xffffffffu, rows, 0) == -2) gone |= 0xffffu;
-        if (__shfl_sync(0xffffffffu, rows, 1) == -2) gone |= 0xffff0000u;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const bool bad = (vw[i] & 0x7f80u) == 0x7f80u;
-          if (bad) vw[i] = 0;                              // zeros, and a flag for those who see it
-          const uint32_t at = bad ? 1u << (i * kKps + key0) : 0u;
-          nan[0] |= __reduce_or_sync(0xffffffffu, half == 0 ? at : 0u);
-          nan[1] |= __reduce_or_sync(0xffffffffu, half == 1 ? at : 0u);
-        }
-        any = gone | nan[0] | nan[1];
-        if (lane == 0) {
-          flags[j & 3].gone[w] = gone;
-          flags[j & 3].nan0[w] = nan[0];
-          flags[j & 3].nan1[w] = nan[1];
-        }
+      // flags of tile j (those of j - 4 are out of use: V of j - 1 was written after PV of j - 3 ended)
+      if (lane == 0) {
+        TileFlags& f = flags[j & 3];
+        if (kv == 0) f.gone[w] = gone;
+        else f.nan0[w] = nan[0], f.nan1[w] = nan[1];
       }
-      if (lane == 0) flags[j & 3].any[w] = any;
-      uint4 kc1[kSteps], vc1[kSteps];
-      uint32_t kw1[kSteps], vw1[kSteps];
-      if (j + 1 < ntiles) load(next, j + 1, kc1, vc1, kw1, vw1);
-      const int after = j + 2 < ntiles ? find_rows(j + 2) : -1;
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {                     // K, then V: one copy of the code for the instruction cache
-        if (u >= 1)
-          ok = __all_sync(0xffffffffu, wait_phase((kv ? v_empty : k_empty) + s, (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
-        if (!ok) break;
-        put(smem + (kv ? L::kVOff : L::kKOff) + s * L::kTile, kc, kw);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive((kv ? v_full : k_full) + s);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) kc[i] = vc[i], kw[i] = vw[i];
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive((kv ? v_full : k_full) + s);
+        mbar_arrive(&raw_empty[re]);
       }
-      if (!ok) break;
-      if (j + 1 < ntiles) {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) kc[i] = kc1[i], vc[i] = vc1[i], kw[i] = kw1[i], vw[i] = vw1[i];
-      }
-      rows = next;
-      next = after;
     }
+  } else if (warp == 13) {
+    // ---------------- copies ----------------
+    const int* table = tables + (int64_t)seq * width;
+    int issued[kEntries] = {};
+    bool ok = true;
+    for (int e = 0; e < 2 * ntiles; ++e) {
+      const int j = e >> 1, re = e % kEntries, u = e / kEntries;
+      // lane i takes the i-th page that the tile touches; runs are whole 16-key tiles of a page
+      const int k0 = j * kBK, last = min(k0 + kBK, (kend + 15) & ~15), page = k0 / bs + lane;
+      const int from = max(k0, page * bs), to = min(last, (page + 1) * bs);
+      const bool mine = lane < kBK / 16 + 1 && from < to;
+      const int blk = mine ? table[page] : 0;
+      const bool bad = mine && (blk < 0 || blk >= nblk);
+      uint32_t gone = 0;
+      if (bad) {
+        record_error(status, kBadIndex);
+        gone = ((1u << ((to - k0) / 16)) - 1u) & ~((1u << ((from - k0) / 16)) - 1u);
+      }
+      gone = __reduce_or_sync(0xffffffffu, gone);
+      const int keys = mine && !bad ? to - from : 0;
+      const int total = __reduce_add_sync(0xffffffffu, keys);
+      if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&raw_empty[re], (u - 1) & 1, abort_v, status, kTimeoutSmemEmpty));
+      if (!ok) break;
+      if (lane == 0) {
+        raw_gone[re] = gone;                               // published by the arrival below
+        mbar_expect_tx(&raw_full[re], (uint32_t)total * (HD / 2 + 2 * L::kHalves));
+      }
+      __syncwarp();
+      if (keys > 0) {
+        const Pages& p = e & 1 ? vp : kp;
+        const size_t row = ((size_t)blk * nkv + kvh) * bs + (from - page * bs);
+        const uint32_t dst = smem_u32(smem) + L::kRawOff + re * L::kRaw;
+        bulk_copy(dst + (from - k0) * (HD / 2), p.codes + row * (HD / 2), keys * (HD / 2), &raw_full[re]);
+        bulk_copy(dst + L::kRawCodes + (from - k0) * 2 * L::kHalves, p.words + row * L::kHalves, keys * 2 * L::kHalves, &raw_full[re]);
+      }
+      issued[re] = u + 1;
+    }
+    // every copy has landed before the block may end
+    for (int re = 0; re < kEntries; ++re)
+      if (issued[re] > 0) mbar_wait(&raw_full[re], (issued[re] - 1) & 1);
   } else if (warp == 12) {
     // ---------------- MMA issuer ----------------
     if (lane == 0 && ntiles > 0) {
       constexpr uint32_t id_s = idesc_f16(kBQ, kBK, false), id_pv = idesc_f16(kBQ, HD, true);
-      const uint32_t qa = smem_u32(smem);
+      // descriptors differ in the address field (16-byte units) only
+      const uint64_t dq = desc_kmajor(smem_u32(smem)), dk = desc_kmajor(smem_u32(smem + L::kKOff)),
+                     dv = desc_mnmajor(smem_u32(smem + L::kVOff), L::kHalf);
       bool ok = wait_phase(q_full, 0, abort_v, status, kTimeoutTmaFull);
       auto issue_s = [&](int t, int j) {
         const int s = j & 1;
         if (!wait_phase(&k_full[s], (j >> 1) & 1, abort_v, status, kTimeoutTmaFull)) return false;
         fence_after();
-        const uint32_t ka = smem_u32(smem + L::kKOff + s * L::kTile);
+        const uint64_t qt = dq + t * (L::kTile / 16), kt = dk + s * (L::kTile / 16);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          mma(tmem + t * 128, desc_kmajor(qa + t * L::kTile + (k / 4) * L::kHalf + (k % 4) * 32),
-              desc_kmajor(ka + (k / 4) * L::kHalf + (k % 4) * 32), id_s, k != 0);
+          mma(tmem + t * 128, qt + ((k / 4) * L::kHalf + (k % 4) * 32) / 16, kt + ((k / 4) * L::kHalf + (k % 4) * 32) / 16,
+              id_s, k != 0);
         commit(&s_full[t]);
         if (t == 1 || j >= nt[1]) commit(&k_empty[s]);     // the last S that reads this K tile
         return true;
@@ -293,10 +302,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         if (!wait_phase(&p_full[t], j & 1, abort_v, status, kTimeoutAccum)) return false;
         if (!wait_phase(&v_full[s], (j >> 1) & 1, abort_v, status, kTimeoutTmaFull)) return false;
         fence_after();
-        const uint32_t va = smem_u32(smem + L::kVOff + s * L::kTile);
+        const uint64_t vt = dv + s * (L::kTile / 16);
 #pragma unroll
         for (int k = 0; k < kBK / 16; ++k)
-          mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, desc_mnmajor(va + k * 16 * 128, L::kHalf), id_pv, (j | k) != 0);
+          mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vt + k * 16 * 128 / 16, id_pv, (j | k) != 0);
         if (t == 1 || j >= nt[1]) commit(&v_empty[s]);
         return true;
       };
@@ -340,19 +349,30 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     const uint32_t tmem_s = tmem + t * 128 + base, tmem_o = tmem + 256 + t * 128 + base;
     float m_used = -INFINITY, l = 0.f;
     bool nan0 = false, nan1 = false, ok = true;
+    // NaN groups of V(jj) that this row sees
+    auto note_nan = [&](int jj) {
+      const TileFlags& f = flags[jj & 3];
+      const uint4 a = *reinterpret_cast<const uint4*>(f.nan0), b = *reinterpret_cast<const uint4*>(f.nan1);
+      if ((a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) == 0u) return;
+      for (int c = 0; c < 4; ++c) {
+        const int n = limit - jj * kBK - c * 32;
+        const uint32_t seen = n >= 32 ? ~0u : n <= 0 ? 0u : ~(~0u << n);
+        nan0 |= (f.nan0[c] & seen) != 0u;
+        nan1 |= (f.nan1[c] & seen) != 0u;
+      }
+    };
     for (int j = 0; j < nt[t]; ++j) {
       ok = __all_sync(0xffffffffu, wait_phase(&s_full[t], j & 1, abort_v, status, kTimeoutAccum));
       if (!ok) break;
       fence_after();
       const int k0 = j * kBK;
-      const TileFlags& f = flags[j & 3];
-      const uint4 any = *reinterpret_cast<const uint4*>(f.any);
-      const bool flagged = (any.x | any.y | any.z | any.w) != 0u;
-      const bool inside = !flagged && k0 + kBK <= warp_limit;
+      if (j > 0) note_nan(j - 1);                          // complete: S of this tile was issued after PV of that one
+      const uint4 gone = *reinterpret_cast<const uint4*>(flags[j & 3].gone);
+      const bool inside = (gone.x | gone.y | gone.z | gone.w) == 0u && k0 + kBK <= warp_limit;
       // keys of chunk c that this row does not see, as a bit mask
       auto hidden = [&](int c) {
         const int n = limit - k0 - c * 32;
-        return (n >= 32 ? 0u : n <= 0 ? 0xffffffffu : ~0u << n) | (flagged && ((const volatile uint32_t*)f.any)[c] ? ((const volatile uint32_t*)f.gone)[c] : 0u);
+        return (n >= 32 ? 0u : n <= 0 ? 0xffffffffu : ~0u << n) | flags[j & 3].gone[c];
       };
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
@@ -362,10 +382,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         tmem_wait_ld();
         if (!inside) {
           const uint32_t h = hidden(c);
-          if (flagged && ((const volatile uint32_t*)f.any)[c]) {
-            nan0 |= (((const volatile uint32_t*)f.nan0)[c] & ~h) != 0u;
-            nan1 |= (((const volatile uint32_t*)f.nan1)[c] & ~h) != 0u;
-          }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (h >> e & 1u) x[e] = 0xff800000u;
@@ -426,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     fence_after();
     uint4* dst = reinterpret_cast<uint4*>(out + row * HD);
     if (done) {
+      note_nan(nt[t] - 1);
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int c = 0; c < HD; c += 16) {
