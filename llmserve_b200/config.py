@@ -21,6 +21,10 @@ are grouped at the end:
 * ``speculative_cuda_graphs`` -- capture the greedy EAGLE3 chain step (drafts, packed verify,
                               acceptance) in CUDA graphs per batch bucket; off by default.
 
+* ``kv_cache_dtype``       -- ``"auto"`` keeps K/V in the model's dtype; ``"int4"`` holds the target's pool
+                              in 4-bit pages (4.25 bits per element, ``ops.kv_int4``); an EAGLE3
+                              draft's own pool stays in the model's dtype.
+
 ``awq_backend="triton"`` is accepted for compatibility and runs the sm_100a W4A16 kernel.
 """
 import json
@@ -107,6 +111,7 @@ class Config:
     rpc_channel: str | None = None
     overlap_decode: bool = True
     speculative_cuda_graphs: bool = False
+    kv_cache_dtype: str = "auto"
     pd_role: str = ""          # internal: "decode" exports its KV pools to the prefill ranks
 
     def __post_init__(self):
@@ -147,6 +152,15 @@ class Config:
                 AWQRuntimeConfig.from_hf_config(self.hf_config),
                 execution_backend=self.awq_backend,
             )
+        if self.kv_cache_dtype not in ("auto", "int4"):
+            raise ValueError("kv_cache_dtype must be 'auto' or 'int4'")
+        if self.kv_cache_dtype == "int4":
+            if self.hf_config.head_dim not in (64, 128):
+                raise ValueError("kv_cache_dtype='int4' needs head_dim 64 or 128")
+            if self.device == "cuda" and self.hf_config.dtype != torch.bfloat16:
+                raise ValueError("kv_cache_dtype='int4' runs bfloat16 models")
+            if self.pd_disaggregation or self.pd_role:
+                raise ValueError("kv_cache_dtype='int4' does not support prefill/decode disaggregation")
         self.max_model_len = min(self.max_model_len, self.hf_config.max_position_embeddings)
         if self.pd_disaggregation:
             if not self.pd_prefill_devices or not self.pd_decode_devices:

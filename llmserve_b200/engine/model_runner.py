@@ -5,6 +5,9 @@ sizing ``:186-229``, metadata ``:258-338``, graphs ``:383-418``).  Differences b
 
 * KV pools are ``k/v_cache[L, blocks, kv_heads, block_size, head_dim]`` (see ``ops.attention``)
   plus an EAGLE3 draft pool with the same block ids;
+* ``kv_cache_dtype="int4"`` holds the target's pools in 4-bit pages (``ops.kv_int4``);
+* on the GPU a prefill or eager decode step sends request lengths and block ids, and one kernel
+  fills positions, slots and block tables (``ops.step_maps``);
 * prefill metadata carries per-sequence key lengths for the paged varlen kernel and the LM-head
   row selection; every prefill reads K/V from the pool (one kernel path for plain, chunked,
   prefix-cached and verify batches);
@@ -27,7 +30,9 @@ from llmserve_b200.engine.scheduler import SchedulerOutput
 from llmserve_b200.engine.sequence import Sequence
 from llmserve_b200.models.qwen3 import Qwen3ForCausalLM
 from llmserve_b200.ops import attention as attn_ops
+from llmserve_b200.ops import kv_int4
 from llmserve_b200.ops import sampling as sampling_ops
+from llmserve_b200.ops import step_maps
 from llmserve_b200.ops._ext import LaunchCounter
 from llmserve_b200.parallel import state as tp
 from llmserve_b200.utils.context import reset_context, set_context
@@ -250,11 +255,20 @@ class ModelRunner:
         hf = self.hf_config
         nkv = hf.num_key_value_heads // self.world_size
         esize = torch.tensor([], dtype=self.dtype).element_size()
-        per = 2 * hf.num_hidden_layers * self.block_size * nkv * hf.head_dim * esize
+        row = hf.head_dim * esize
+        if self.config.kv_cache_dtype == "int4":
+            row = hf.head_dim // 2 + 2 * (hf.head_dim // kv_int4.GROUP)
+        per = 2 * hf.num_hidden_layers * self.block_size * nkv * row
         if self.draft_model is not None:
             d = self.draft_model
             per += 2 * self.block_size * d.num_kv_heads * d.head_dim * esize
         return per
+
+    def _target_pool(self, shape):
+        """One empty target pool (K or V) ``[layers, blocks, kv_heads, block_size, head_dim]``."""
+        if self.config.kv_cache_dtype == "int4":
+            return kv_int4.Int4Pages.zeros(shape, self.device)
+        return torch.zeros(shape, dtype=self.dtype, device=self.device)
 
     def _bind_pools(self, k_cache, v_cache, dk=None, dv=None):
         empty = torch.tensor([])
@@ -278,15 +292,14 @@ class ModelRunner:
         need = -(-seq_len // self.block_size)
         nkv = hf.num_key_value_heads // self.world_size
         shape = (hf.num_hidden_layers, need * num_seqs, nkv, self.block_size, hf.head_dim)
-        k = torch.zeros(shape, dtype=self.dtype, device=self.device)
-        v = torch.zeros_like(k)
+        k, v = self._target_pool(shape), self._target_pool(shape)
         dk = dv = None
         if self.draft_model is not None:
             d = self.draft_model
             dk = torch.zeros(need * num_seqs, d.num_kv_heads, self.block_size, d.head_dim,
                              dtype=self.dtype, device=self.device)
             dv = torch.zeros_like(dk)
-        self.warmup_pool_bytes = sum(t.numel() * t.element_size() for t in (k, v, dk, dv) if t is not None)
+        self.warmup_pool_bytes = sum(t.nbytes for t in (k, v, dk, dv) if t is not None)
         self._bind_pools(k, v, dk, dv)
         seqs = [Sequence([0] * seq_len) for _ in range(num_seqs)]
         for i, s in enumerate(seqs):
@@ -328,8 +341,7 @@ class ModelRunner:
         if cfg.pd_role == "decode":
             self.k_cache, self.v_cache = self._exportable_pools(shape, "kv")
         else:
-            self.k_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
-            self.v_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
+            self.k_cache, self.v_cache = self._target_pool(shape), self._target_pool(shape)
         self.draft_k_cache = self.draft_v_cache = None
         if self.draft_model is not None:
             d = self.draft_model
@@ -467,7 +479,7 @@ class ModelRunner:
             if key not in seen:
                 seen.add(key)
                 model_bytes += t.untyped_storage().nbytes()
-        kv_bytes = (self.k_cache.numel() + self.v_cache.numel()) * self.k_cache.element_size()
+        kv_bytes = self.k_cache.nbytes + self.v_cache.nbytes
         out = {
             "model_runtime_bytes": model_bytes,
             "kv_cache_bytes": kv_bytes,
@@ -525,30 +537,49 @@ class ModelRunner:
         table = np.asarray(seq.block_table, dtype=np.int64)
         return table[pos // self.block_size] * self.block_size + pos % self.block_size
 
+    def _device_maps(self, seqs, q_lens: list[int], k_lens: list[int]):
+        """The step's maps built on the GPU: one copy of lengths and block ids, one kernel.  Returns
+        ``(maps, key lengths)``."""
+        bsz, n = self.block_size, len(seqs)
+        blocks = [-(-k // bsz) for k in k_lens]
+        a = np.empty(2 * n + sum(blocks), dtype=np.int32)
+        a[:n], a[n:2 * n] = q_lens, k_lens
+        at = 2 * n
+        for s, m in zip(seqs, blocks):
+            a[at:at + m] = s.block_table[:m]
+            at += m
+        self.h2d_bytes += a.nbytes
+        t = _to_device(a, torch.int32, self.device)
+        maps = step_maps.build_step_maps(t[:n], t[n:2 * n], t[2 * n:], bsz, sum(q_lens), max(1, max(blocks)))
+        return maps, t[n:2 * n]
+
     def prepare_prefill(self, seqs: list[Sequence], decode_seqs: list[Sequence] | None = None):
         decode_ids = {s.seq_id for s in (decode_seqs or [])}
-        ids, pos, slots = [], [], []
-        cu_q, cu_k, lens_k, last = [0], [0], [], []
-        max_q = max_k = 0
+        ids, starts, q_lens, lens_k = [], [], [], []
         for s in seqs:
             if s.seq_id in decode_ids:
                 start, q = len(s) - 1, 1
             else:
                 start, q = min(s.num_cached_tokens, len(s) - 1), s.num_scheduled_tokens
-            end = start + q
-            ids.extend(s.token_ids[start:end])
-            pos.extend(range(start, end))
-            slots.append(self._slots(s, start, end))
-            cu_q.append(cu_q[-1] + q)
-            cu_k.append(cu_k[-1] + end)
-            lens_k.append(end)
-            last.append(cu_q[-1] - 1)
-            max_q, max_k = max(max_q, q), max(max_k, end)
+            ids.extend(s.token_ids[start:start + q])
+            starts.append(start)
+            q_lens.append(q)
+            lens_k.append(start + q)
         d = self.device
-        slot_arr = np.concatenate(slots)
+        max_q, max_k = max(q_lens), max(lens_k)
         if self.config.debug_bounds_checks:
-            for s, sl, end in zip(seqs, slots, lens_k):
-                self.check_bounds([s], np.arange(end - len(sl), end), sl)
+            for s, start, end in zip(seqs, starts, lens_k):
+                self.check_bounds([s], np.arange(start, end), self._slots(s, start, end))
+        if self.is_cuda and len(seqs) <= step_maps.MAX_REQUESTS:
+            self.h2d_bytes += 8 * len(ids)
+            maps, seqlens_k = self._device_maps(seqs, q_lens, lens_k)
+            set_context(True, cu_seqlens_q=maps.cu_seqlens_q, max_seqlen_q=max_q, max_seqlen_k=max_k,
+                        slot_mapping=maps.slot_mapping, block_tables=maps.block_tables, seqlens_k=seqlens_k,
+                        last_token_indices=maps.last_token_indices, decode_workspace=self.decode_workspace)
+            return _to_device(ids, torch.int64, d), maps.positions
+        cu_q, cu_k = np.cumsum([0] + q_lens), np.cumsum([0] + lens_k)
+        pos = np.concatenate([np.arange(a, b) for a, b in zip(starts, lens_k)])
+        slot_arr = np.concatenate([self._slots(s, a, b) for s, a, b in zip(seqs, starts, lens_k)])
         self.h2d_bytes += 16 * len(ids) + 4 * len(slot_arr) + 16 * len(seqs) + 8
         set_context(
             True,
@@ -558,7 +589,7 @@ class ModelRunner:
             slot_mapping=_to_device(slot_arr, torch.int32, d),
             block_tables=self.prepare_block_tables(seqs),
             seqlens_k=_to_device(lens_k, torch.int32, d),
-            last_token_indices=_to_device(last, torch.int64, d),
+            last_token_indices=_to_device(cu_q[1:] - 1, torch.int64, d),
             decode_workspace=self.decode_workspace,
         )
         return _to_device(ids, torch.int64, d), _to_device(pos, torch.int64, d)
@@ -566,15 +597,21 @@ class ModelRunner:
     def prepare_decode(self, seqs: list[Sequence]):
         n = len(seqs)
         ids = np.empty(n, dtype=np.int64)
-        pos = np.empty(n, dtype=np.int64)
-        slots = np.empty(n, dtype=np.int32)
         lens = np.empty(n, dtype=np.int32)
         for i, s in enumerate(seqs):
-            L = len(s)
-            ids[i], pos[i], lens[i] = s.last_token, L - 1, L
-            slots[i] = s.block_table[(L - 1) // self.block_size] * self.block_size + (L - 1) % self.block_size
+            ids[i], lens[i] = s.last_token, len(s)
         d = self.device
-        self.check_bounds(seqs, pos, slots)
+        pos = lens.astype(np.int64) - 1
+        if not self.is_cuda or n > step_maps.MAX_REQUESTS or self.config.debug_bounds_checks:
+            slots = np.array([s.block_table[p // self.block_size] * self.block_size + p % self.block_size
+                              for s, p in zip(seqs, pos.tolist())], dtype=np.int32)
+            self.check_bounds(seqs, pos, slots)
+        if self.is_cuda and n <= step_maps.MAX_REQUESTS:
+            self.h2d_bytes += ids.nbytes
+            maps, context_lens = self._device_maps(seqs, [1] * n, lens.tolist())
+            set_context(False, slot_mapping=maps.slot_mapping, context_lens=context_lens, block_tables=maps.block_tables,
+                        decode_workspace=self.decode_workspace)
+            return _to_device(ids, torch.int64, d), maps.positions
         self.h2d_bytes += ids.nbytes + pos.nbytes + slots.nbytes + lens.nbytes
         set_context(False, slot_mapping=_to_device(slots, torch.int32, d), context_lens=_to_device(lens, torch.int32, d),
                     block_tables=self.prepare_block_tables(seqs), decode_workspace=self.decode_workspace)

@@ -3,12 +3,14 @@
 The QK RMSNorm, RoPE and the K/V store into the pool run as one kernel; then prefill (varlen
 paged) or decode (split-KV) attention reads the pool.  In tree-verify mode the nodes' K/V are not
 stored: they are captured in ``tree_k``/``tree_v`` and attended with the ancestor mask, and the
-accepted path is committed afterwards by ``ops.kv.commit_tree_kv``.
+accepted path is committed afterwards by ``ops.kv.commit_tree_kv``.  A pool of 4-bit pages
+(``kv_int4.Int4Pages``) takes the same steps through the operators of ``ops.kv_int4``.
 """
 import torch
 from torch import nn
 
 from llmserve_b200.ops import attention as attn_ops
+from llmserve_b200.ops import kv_int4
 from llmserve_b200.ops import rope as rope_ops
 from llmserve_b200.utils.context import get_context
 
@@ -30,10 +32,13 @@ class Attention(nn.Module):
                                                    None, None, None, self.num_heads, self.num_kv_heads,
                                                    self.head_dim)
             self.tree_k, self.tree_v = k.contiguous(), v.contiguous()
-            o = attn_ops.tree_attention(q, self.k_cache, self.v_cache, ctx.tree_block_table,
-                                        ctx.tree_prefix_len, self.tree_k, self.tree_v,
-                                        ctx.tree_attention_mask, self.scale, ctx.tree_mask_bits)
+            attend = kv_int4.tree_attention_int4 if isinstance(self.k_cache, kv_int4.Int4Pages) else attn_ops.tree_attention
+            o = attend(q, self.k_cache, self.v_cache, ctx.tree_block_table,
+                       ctx.tree_prefix_len, self.tree_k, self.tree_v, ctx.tree_attention_mask, self.scale,
+                       ctx.tree_mask_bits)
             return o.reshape(T, -1)
+        if isinstance(self.k_cache, kv_int4.Int4Pages):
+            return self._forward_int4(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, ctx).reshape(T, -1)
         q, _, _ = rope_ops.qkv_norm_rope_store(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps,
                                                self.k_cache, self.v_cache, ctx.slot_mapping,
                                                self.num_heads, self.num_kv_heads, self.head_dim)
@@ -48,3 +53,16 @@ class Attention(nn.Module):
             o = attn_ops.decode_attention(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.context_lens,
                                           self.scale, ctx.decode_workspace)
         return o.reshape(T, -1)
+
+    def _forward_int4(self, qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, ctx) -> torch.Tensor:
+        q = kv_int4.qkv_norm_rope_store_int4(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, self.k_cache,
+                                             self.v_cache, ctx.slot_mapping, self.num_heads, self.num_kv_heads,
+                                             self.head_dim)
+        if ctx.is_prefill and ctx.uniform_q:
+            return kv_int4.verify_attention_int4(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.seqlens_k,
+                                                 self.scale, ctx.uniform_q, ctx.decode_workspace)
+        if ctx.is_prefill:
+            return kv_int4.prefill_attention_int4(q, self.k_cache, self.v_cache, ctx.cu_seqlens_q, ctx.seqlens_k,
+                                                  ctx.block_tables, self.scale, ctx.max_seqlen_q)
+        return kv_int4.decode_attention_int4(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.context_lens,
+                                             self.scale, ctx.decode_workspace)

@@ -43,7 +43,9 @@ using namespace umma;
 
 constexpr int kBQ = 128;                  // rows of a tile (UMMA M)
 constexpr int kBK = 128;                  // keys of a tile
-constexpr int kThreads = 14 * 32;
+constexpr int kDeq = 4;                   // dequantising warps, 32 keys of a tile each
+constexpr int kMmaWarp = 8 + kDeq, kCopyWarp = kMmaWarp + 1;
+constexpr int kThreads = (kCopyWarp + 1) * 32;
 constexpr int kEntries = 3;               // ring of packed tiles
 constexpr float kRescaleLog2 = 8.f;
 
@@ -82,6 +84,32 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two fp32 at a time (one instruction)
+__device__ __forceinline__ uint64_t join2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
   uint32_t y;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
@@ -101,7 +129,7 @@ __device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t 
 // What softmax has to know of a 128-key tile beyond its position, a bit per key: keys that are not there
 // (known when K is), and those whose V group 0 / 1 is NaN (known when V is).
 struct TileFlags {
-  uint32_t gone[4], nan0[4], nan1[4];
+  uint32_t gone[4], nan0[4], nan1[4];      // per dequantising warp
 };
 
 template <int HD>
@@ -114,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-           *s_full = bars + 9, *p_full = bars + 11, *drain = bars + 13, *raw_full = bars + 14,
+           *s_full = bars + 9, *p_full = bars + 11, *p_half = bars + 13, *drain = bars + 15, *raw_full = bars + 16,
            *raw_empty = raw_full + kEntries;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + kEntries);
   volatile uint32_t* raw_gone = tmem_slot + 1;             // 16-key tiles of an entry that are not there
@@ -142,25 +170,39 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   }
   const int kend = max(kend_t[0], kend_t[1]), ntiles = max(nt[0], nt[1]);
 
+  // the softmax warps' query rows, on their way while the barriers are set up
+  uint4 qv[HD / 8];
+  if (warp < 8) {
+    constexpr int kPieces = HD / 8;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int rr = (warp & 3) * 32 + i * (32 / kPieces) + lane / kPieces;
+      const int qi = first + (warp >> 2) * per_tile + rr / G;
+      qv[i] = make_uint4(0, 0, 0, 0);
+      if (rr < per_tile * G && qi < q_len)
+        qv[i] = __ldg(reinterpret_cast<const uint4*>(q + ((size_t)(q0 + qi) * nh + kvh * G + rr % G) * HD) + lane % kPieces);
+    }
+  }
   if (threadIdx.x == 0) {
     abort_flag = 0;
     mbar_init(q_full, 8);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 4);
+      mbar_init(&k_full[s], kDeq);
       mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 4);
+      mbar_init(&v_full[s], kDeq);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
+      mbar_init(&p_half[s], 4);
     }
     for (int e = 0; e < kEntries; ++e) {
       mbar_init(&raw_full[e], 1);
-      mbar_init(&raw_empty[e], 4);
+      mbar_init(&raw_empty[e], kDeq);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -169,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   fence_after();
   const uint32_t tmem = *tmem_slot;                        // S (then P) of tile t at 128 t, O at 256 + 128 t
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8 && warp < kMmaWarp) {
     // ---------------- dequantisation ----------------
     constexpr int kCpk = HD / 32;                          // 16-byte chunks of a key
     constexpr int kKps = 32 / kCpk;                        // keys of a step
@@ -196,9 +238,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
       const uint32_t gone16 = raw_gone[re] >> (w * 2) & 3u;
       const uint32_t gone = (gone16 & 1u ? 0xffffu : 0u) | (gone16 & 2u ? 0xffff0000u : 0u);
       const int left = kend - j * kBK - w * 32;
-      const uint32_t zero = gone | (left >= 32 ? 0u : left <= 0 ? 0xffffffffu : ~0u << left);
+      const uint32_t zero = gone | (left >= 32 ? 0u : left <= 0 ? ~0u : ~0u << left);
       uint32_t nan[2] = {0, 0};
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < 32 / kKps; ++i) {
         const int in_warp = lane / kCpk + i * kKps;
         const uint2 c0 = *reinterpret_cast<const uint2*>(raw + src0 + i * kKps * (HD / 2));
@@ -236,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         mbar_arrive(&raw_empty[re]);
       }
     }
-  } else if (warp == 13) {
+  } else if (warp == kCopyWarp) {
     // ---------------- copies ----------------
     const int* table = tables + (int64_t)seq * width;
     int issued[kEntries] = {};
@@ -276,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     // every copy has landed before the block may end
     for (int re = 0; re < kEntries; ++re)
       if (issued[re] > 0) mbar_wait(&raw_full[re], (issued[re] - 1) & 1);
-  } else if (warp == 12) {
+  } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
     if (lane == 0 && ntiles > 0) {
       constexpr uint32_t id_s = idesc_f16(kBQ, kBK, false), id_pv = idesc_f16(kBQ, HD, true);
@@ -299,13 +341,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
       };
       auto issue_pv = [&](int t, int j) {
         const int s = j & 1;
-        if (!wait_phase(&p_full[t], j & 1, abort_v, status, kTimeoutAccum)) return false;
+        if (!wait_phase(&p_half[t], j & 1, abort_v, status, kTimeoutAccum)) return false;
         if (!wait_phase(&v_full[s], (j >> 1) & 1, abort_v, status, kTimeoutTmaFull)) return false;
-        fence_after();
         const uint64_t vt = dv + s * (L::kTile / 16);
 #pragma unroll
-        for (int k = 0; k < kBK / 16; ++k)
+        for (int k = 0; k < kBK / 16; ++k) {
+          if (k == kBK / 32 && !wait_phase(&p_full[t], j & 1, abort_v, status, kTimeoutAccum)) return false;
+          if (k % (kBK / 32) == 0) fence_after();
           mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vt + k * 16 * 128 / 16, id_pv, (j | k) != 0);
+        }
         if (t == 1 || j >= nt[1]) commit(&v_empty[s]);
         return true;
       };
@@ -327,16 +371,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     const int qi = first + t * per_tile + r / G, head = kvh * G + r % G;
     const bool live = r < per_tile * G && qi < q_len;
     const size_t row = (size_t)(q0 + (live ? qi : 0)) * nh + head;
-    // Q row into the tile, 8 dims at a time in the order 0 4 1 5 2 6 3 7; rows without a query are zeros
+    // Q rows of this warp into the tile, 8 dims at a time in the order 0 4 1 5 2 6 3 7; rows without a query
+    // are zeros
     {
-      const uint4* src = reinterpret_cast<const uint4*>(q + row * HD);
-      uint8_t* dst = smem + t * L::kTile + r * 128;
+      constexpr int kPieces = HD / 8;
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = live ? src[c] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (c / 8) * L::kHalf + (((c % 8) ^ (r & 7)) << 4)) =
-            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                       __byte_perm(v.y, v.w, 0x7632));
+      for (int i = 0; i < kPieces; ++i) {
+        const int rr = (warp & 3) * 32 + i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+        *reinterpret_cast<uint4*>(smem + t * L::kTile + (c / 8) * L::kHalf + rr * 128 + (((c % 8) ^ (rr & 7)) << 4)) =
+            make_uint4(__byte_perm(qv[i].x, qv[i].z, 0x5410), __byte_perm(qv[i].x, qv[i].z, 0x7632),
+                       __byte_perm(qv[i].y, qv[i].w, 0x5410), __byte_perm(qv[i].y, qv[i].w, 0x7632));
       }
       fence_async_smem();
       __syncwarp();
@@ -374,12 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         const int n = limit - k0 - c * 32;
         return (n >= 32 ? 0u : n <= 0 ? 0xffffffffu : ~0u << n) | flags[j & 3].gone[c];
       };
+      // the next 32 scores are on their way while these are worked on
+      uint32_t xa[32], xb[32];
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32];
-        tmem_ld32(tmem_s + c * 32, x);
-        tmem_wait_ld();
+      auto largest = [&](uint32_t* x, int c) {
         if (!inside) {
           const uint32_t h = hidden(c);
 #pragma unroll
@@ -387,7 +429,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
             if (h >> e & 1u) x[e] = 0xff800000u;
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(x[e]));
+        for (int e = 0; e < 32; e += 2)
+          mx4[e / 2 & 3] = max3(mx4[e / 2 & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+      };
+      tmem_ld32(tmem_s, xa);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        tmem_wait_ld();
+        tmem_ld32(tmem_s + c * 32 + 32, xb);
+        largest(xa, c);
+        tmem_wait_ld();
+        tmem_ld32(tmem_s + (c * 32 + 64) % 128, xa);       // at the end: chunk 0 again, for the exponentials
+        largest(xb, c + 1);
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
       float alpha = 1.f;
@@ -408,33 +461,40 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
         }
       }
       const float neg_m = m_used == -INFINITY ? 0.f : -m_used;      // a row that sees nothing: all P = 0
-      float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t x[32], p[16];
-        tmem_ld32(tmem_s + c * 32, x);
-        tmem_wait_ld();
+      const uint64_t scale2 = join2(scale_log2, scale_log2), neg2 = join2(neg_m, neg_m);
+      uint64_t sum2[2] = {0, 0};
+      auto weights = [&](uint32_t* x, int c) {
         if (!inside) {
           const uint32_t h = hidden(c);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (h >> e & 1u) x[e] = 0xff800000u;
         }
+        uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float a = ex2(fmaf(__uint_as_float(x[e]), scale_log2, neg_m));
-          const float b = ex2(fmaf(__uint_as_float(x[e + 1]), scale_log2, neg_m));
-          sum4[e & 2] += a;
-          sum4[(e & 2) + 1] += b;
+          const float2 y = split2(fma_pair(join2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, neg2));
+          const float a = ex2(y.x), b = ex2(y.y);
+          sum2[e / 2 & 1] = add_pair(sum2[e / 2 & 1], join2(a, b));
           p[e / 2] = pack2_bf16(a, b);
         }
         tmem_st16(tmem_s + c * 16, p);
+      };
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        tmem_wait_ld();
+        tmem_ld32(tmem_s + c * 32 + 32, xb);
+        weights(xa, c);                                    // P's 16 columns lie in chunks already read
+        tmem_wait_ld();
+        if (c == 0) tmem_ld32(tmem_s + 64, xa);
+        weights(xb, c + 1);
+        tmem_wait_st();                                    // half of P is there: its products may start
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive((c == 0 ? p_half : p_full) + t);
       }
-      l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      const float2 sum = split2(add_pair(sum2[0], sum2[1]));
+      l += sum.x + sum.y;
     }
     // O / l, columns back in order
     const bool done = ok && nt[t] > 0 &&
@@ -465,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   }
   fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }

@@ -11,6 +11,7 @@ bfloat16 pattern of the group's scale ``s`` with the four low mantissa bits repl
 * ``load_kvcache_int4``         -- the rows at given slots as bfloat16 (``slot < 0`` gives zeros).
 * ``qkv_norm_rope_store_int4``  -- one step's projection: QK-norm, RoPE, query out, K/V into the pages.
 * ``decode_attention_int4``     -- one query per sequence; ``verify_attention_int4``: ``nq`` of them.
+* ``tree_attention_int4``       -- EAGLE3 tree verify on a 4-bit prefix.
 * ``prefill_attention_int4``    -- ragged causal chunks, on a cached prefix or without.
 
 On CUDA a slot or block id outside the pool is skipped (its keys are not seen) and recorded for
@@ -224,6 +225,22 @@ def decode_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table
                           workspace=None):
     """One query token per sequence: ``q [B, nh, hd]`` against ``context_lens`` int32 [B] keys."""
     return verify_attention_int4(q, k_pages, v_pages, block_tables, context_lens, scale, 1, workspace)
+
+
+def tree_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table, prefix_len, tree_k, tree_v, tree_mask,
+                        scale, mask_bits=None):
+    """Tree verify on a 4-bit prefix: the sequence's pages are read back once (exact in bfloat16) and
+    ``ops.attention.tree_attention`` runs on the copy."""
+    bs = k_pages.shape[2]
+    n = max(1, -(-prefix_len // bs))
+    if not q.is_cuda:
+        ids = block_table[:n].long()
+        k, v = (dequantise_int4_ref(p.codes[ids], p.words[ids]).to(q.dtype) for p in (k_pages, v_pages))
+    else:
+        slots = (block_table[:n].to(torch.int32)[:, None] * bs + torch.arange(bs, dtype=torch.int32, device=q.device)).flatten()
+        k, v = (x.unflatten(0, (-1, bs)).transpose(1, 2).contiguous() for x in load_kvcache_int4(k_pages, v_pages, slots))
+    table = torch.arange(n, dtype=torch.int32, device=q.device)
+    return attn_ops.tree_attention(q, k, v, table, prefix_len, tree_k, tree_v, tree_mask, scale, mask_bits)
 
 
 def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens_q, seqlens_k, block_tables, scale,

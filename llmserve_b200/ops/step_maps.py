@@ -12,6 +12,9 @@ import torch
 from llmserve_b200.ops._ext import C, status
 
 
+MAX_REQUESTS = 8192      # one block's shared memory holds their prefix sums
+
+
 class StepMaps(NamedTuple):
     cu_seqlens_q: torch.Tensor         # int32 [B + 1]
     positions: torch.Tensor            # int64 [num_tokens]

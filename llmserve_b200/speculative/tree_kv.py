@@ -13,6 +13,7 @@ from collections.abc import Sequence
 import torch
 
 from llmserve_b200.ops import kv as kv_ops
+from llmserve_b200.ops import kv_int4
 
 
 class TreeKVCacheManager:
@@ -56,6 +57,11 @@ class TreeKVCacheManager:
             self._check(node_indices, slot_mapping)
             if self.k_cache is None or self.v_cache is None:
                 raise ValueError("a tree K/V commit needs the target K/V pools")
+            if isinstance(self.k_cache, kv_int4.Int4Pages):
+                for i, layer in enumerate(self.attention_layers):
+                    kv_int4.store_kvcache_int4(layer.tree_k[node_indices], layer.tree_v[node_indices], self.k_cache[i],
+                                               self.v_cache[i], slot_mapping)
+                return
             tree_k = torch.stack([layer.tree_k for layer in self.attention_layers])
             tree_v = torch.stack([layer.tree_v for layer in self.attention_layers])
             nodes = torch.tensor(node_indices, dtype=torch.int32, device=tree_k.device)
