@@ -2,37 +2,32 @@
 //
 // The query rows of one KV head (nq new tokens x heads per KV head) are the narrow side of the tensor
 // core products and the keys and head dims the wide one, with mma.sync and fp32 sums:
-//   S^T [16 keys x 8 rows] = C_K [16 x HD] Q^T        O^T [16 dims x 8 rows] += (C_V - z)^T [16 x 16 keys] W^T
-// so a tile of 16 keys costs 8 rows of padding at most (16 from nine rows on).  A tcgen05 tile would
-// need 128 of them.
+//   S^T [16 keys x 8 rows] = (C_K - z) [16 x HD] Q^T    O^T [16 dims x 8 rows] += (C_V - z)^T [16 x 16 keys] W^T
+// so a tile of 16 keys costs 8 rows of padding at most, where a tcgen05 tile would need 128 of them.  More
+// than eight rows are so many tiles of eight, next to one another in the grid: the second reads the keys
+// from L2.
 //
 // What bounds it next to memory is the integer pipe (64 lanes a clock) that turns nibbles into operands.
-//   K: a byte 0..15 read as e4m3 is c 2^-9 exactly (subnormals and the first binade are one even grid),
-//      so masking alone makes the operand: 3 instructions for 8 codes where a 16-bit form takes 7.  The
-//      query, eight significant bits, becomes two e4m3 terms after scaling the row by a power of two;
-//      values below 2^-10 of the row's largest lose what lies under 2^-17 of it.
-//      s = sum_g sk_g (sum_d q_d c_d - zk_g sum_d q_d)     g: groups of 64 dims
-//   V: 128 + c is a bf16 with c in its low mantissa bits (a mask-or for two nibbles); less 128 + zv of its
-//      key and group it is the exact c - zv.  The other operand is w_jg = p_j sv_jg in bf16, the one
-//      rounding besides the output's.  e4m3 has too few bits for w.
-//
+// A nibble masked where it stands in a 16-bit lane is a bf16 (the patterns up to 255 are an even grid through
+// zero), and a multiply-add by 2^127 turns it into the exact (c - z) / 64 or, four bits up, (c - z) / 4: five
+// integer instructions for eight codes.  The powers of two go into the query and into O's rows.
+//   s = sum_g sk_g sum_d q_d (c_d - z_g), g: groups of 64 dims      w_jg = p_j sv_jg in bf16: the one rounding
+// besides the output's.
 // A warp's operand layout asks K for 8 dims of a key (a code word as it lies) and V for pairs of keys (one
 // PRMT joins the half words of two rows): neither needs a shuffle, and the order of dims or keys inside a
 // product is free as long as both operands share it.
 //
-// One producer warp copies 128-key chunks (codes and words of K and V, a contiguous run per page) into
-// a ring with bulk copies; four consumer warps take 32 keys of every chunk and never meet until a
-// segment ends.  Work is the list of (sequence, KV head, chunk), cut into equal contiguous shares over a
-// grid that fills the GPU once, whatever the lengths: lengths are read on the device, so one captured
-// launch serves any batch.  A (sequence, head) that is cut leaves fp32 partials; the block that
-// finishes last merges them in their order (results do not depend on who is last) and resets the
-// counter.  Bound by memory for long contexts, by instruction issue (about 280 for 16 keys a warp) just
-// behind it.
+// A warp takes 32 keys of every 128-key chunk and copies them itself, bulk copies into a ring of its own (a
+// producer warp would cost registers that four more computing warps need); the four warps of a block
+// meet when a segment ends.  Work is the list of (sequence, KV head, chunk), cut into equal contiguous
+// shares over a grid that fills the GPU once, whatever the lengths: lengths are read on the device, so one
+// captured launch serves any batch.  A (sequence, head) that is cut leaves fp32 partials; the block that
+// finishes last merges them in their order (results do not depend on who is last) and resets the counter.
+// Where every (sequence, head) can have a block and none is more than kCutCost chunks above the equal share,
+// nothing is cut: leaving and merging a piece costs about as much as that many chunks.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-
-#include <cuda_fp16.h>
 
 #include <cmath>
 #include <type_traits>
@@ -49,25 +44,27 @@ namespace {
 using namespace int4;
 using umma::wait_phase;
 
-constexpr int kChunk = 128;               // keys of a ring stage, the unit of work
-constexpr int kWarps = 4;                 // consumer warps
+constexpr int kChunk = 128;               // keys of a unit of work
+constexpr int kWarps = 4;
 constexpr int kWarpKeys = kChunk / kWarps;
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBlocksPerSm = 4;           // 128 registers a thread
+constexpr int kRows = 8;                  // query rows of a block
+constexpr int kCutCost = 3;
 constexpr float kRescaleLog2 = 8.f;
 
-template <int HD, int NT>
+template <int HD>
 struct DecLayout {
   static constexpr int kGroups = HD / kGroup;
-  static constexpr int kStages = 3;
-  static constexpr int kBlocks = NT == 2 ? 2 : 3;          // resident blocks per SM that registers are held to
-  static constexpr int kCodes = kChunk * HD / 2;           // bytes of one tensor's codes in a stage
-  static constexpr int kWords = kChunk * kGroups * 2;
-  static constexpr int kStage = 2 * kCodes + 2 * kWords;
+  static constexpr int kStages = HD == 128 ? 2 : 4;        // of a warp's ring
+  static constexpr int kCodes = kWarpKeys * HD / 2;        // bytes of one tensor's codes in a stage
+  static constexpr int kWords = kWarpKeys * kGroups * 2;
+  static constexpr int kStage = 2 * kCodes + 2 * kWords;   // K codes, V codes, K words, V words
   static constexpr int kRow = HD + 4;                      // floats of a merge row (padded)
-  static constexpr int kMergeOff = kStages * kStage;
-  static constexpr int kMlOff = kMergeOff + kWarps * 8 * NT * kRow * 4;
-  static constexpr int kBarOff = kMlOff + kWarps * 8 * NT * 8;
-  static constexpr int kBytes = kBarOff + 128;
+  static constexpr int kMergeOff = kWarps * kStages * kStage;
+  static constexpr int kMlOff = kMergeOff + kWarps * kRows * kRow * 4;
+  static constexpr int kBarOff = kMlOff + kWarps * kRows * 8;
+  static constexpr int kBytes = kBarOff + kWarps * kStages * 8;
 };
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -86,46 +83,35 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// (x & mask) | bits, one instruction
-__device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t bits) {
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t x, uint32_t m, uint32_t z) {
   uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(z));
   return y;
 }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t x, uint32_t z) {
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t x, uint32_t m) {
   uint32_t y;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(m));
   return y;
 }
-__device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t z) {
-  uint32_t y;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
-  return y;
+// The patterns 0 .. 255 of bf16 (subnormals and the first binade) are one even grid: n 2^-133.  So a nibble
+// masked where it stands is c 2^-133 or, four bits up, c 2^-129, and one multiply-add by 2^127 makes the
+// exact (c - z) / 64 or (c - z) / 4.
+constexpr uint32_t kUp = 0x7f007f00u;      // 2^127 twice
+// zero codes of a pair of 16-bit lanes (in their low four bits) as -z / 64 and -z / 4
+struct Zeros {
+  uint32_t low, high;
+};
+__device__ __forceinline__ Zeros zeros(uint32_t w) {
+  const uint32_t low = mul_bf16x2(w & 0x000f000fu, kUp | 0x80008000u);
+  return {low, mul_bf16x2(low, 0x41804180u)};
 }
-__device__ __forceinline__ uint32_t fma_f16x2(uint32_t x, uint32_t m, uint32_t z) {
-  uint32_t y;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(z));
-  return y;
-}
-// nibbles s and s + 4 of a word as the bf16 pair (128 + low, 128 + high)
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int s) { return mask_or(w >> (4 * s), 0x000f000fu, 0x43004300u); }
-// the eight nibbles of a word less z as fp16 pairs (s, s + 4): nz = -(1024 + z) twice, nz64 = -(64 + z) twice
-__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t nz, uint32_t nz64, uint32_t* y) {
+// nibbles (s, s + 4) of a word less the lanes' zero codes: /64 for even s, /4 for odd s
+__device__ __forceinline__ void codes_bf16(uint32_t w, const Zeros& z, uint32_t* y) {
   const uint32_t h = w >> 8;
-  y[0] = add_f16x2(mask_or(w, 0x000f000fu, 0x64006400u), nz);
-  y[1] = fma_f16x2(mask_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, nz64);      // (1024 + 16 c) / 16
-  y[2] = add_f16x2(mask_or(h, 0x000f000fu, 0x64006400u), nz);
-  y[3] = fma_f16x2(mask_or(h, 0x00f000f0u, 0x64006400u), 0x2c002c00u, nz64);
-}
-__device__ __forceinline__ uint32_t pack2_f16(float a, float b) {
-  __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&v);
+  y[0] = fma_bf16x2(w & 0x000f000fu, kUp, z.low);
+  y[1] = fma_bf16x2(w & 0x00f000f0u, kUp, z.high);
+  y[2] = fma_bf16x2(h & 0x000f000fu, kUp, z.low);
+  y[3] = fma_bf16x2(h & 0x00f000f0u, kUp, z.high);
 }
 
 struct Args {
@@ -138,8 +124,9 @@ struct Args {
   float* part_ml;
   int* counters;
   int* status;
-  float scale_log2;
+  float scale_log2;            // 16 times the scale, for scores in the log2 domain
   int width, B, nq, nh, nkv, bs, nblk, max_splits, row_tiles;
+  uint32_t page_magic;         // ceil(2^32 / (bs / 16)); 0 for blocks of 16
 };
 
 __device__ __forceinline__ int key_count(const Args& a, int b) {
@@ -149,23 +136,36 @@ __device__ __forceinline__ int chunk_count(const Args& a, int b) { return (key_c
 
 // This block's share [c0, c1) of all chunks and where it starts; the same in every lane of a warp.
 struct Share {
-  int c0, c1, total;
+  int c0, c1;
   int b;             // sequence of chunk c0
   int before;        // chunks of all heads before sequence b
 };
-__device__ __forceinline__ int share_begin(int total, int grid, int i) { return (int)((int64_t)total * i / grid); }
+// All chunks, and the blocks they are dealt to (0: a block per (sequence, head), nothing cut).
+struct Deal {
+  int total, grid;
+};
+__device__ __forceinline__ int share_begin(const Deal& d, int i) { return (int)((int64_t)d.total * i / d.grid); }
 
-__device__ __forceinline__ Share find_share(const Args& a, int lane, int& grid) {
-  int sum = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) sum += b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
-  Share s;
-  s.total = __reduce_add_sync(0xffffffffu, sum) * a.nkv;
-  grid = min((int)gridDim.x, s.total);
-  s.c0 = s.c1 = s.b = s.before = 0;
-  if ((int)blockIdx.x >= grid) return s;
-  s.c0 = share_begin(s.total, grid, blockIdx.x);
-  s.c1 = share_begin(s.total, grid, blockIdx.x + 1);
-  const int want = s.c0 / a.nkv;          // the sequence whose per-head chunks hold this one
+__device__ __forceinline__ Share find_share(const Args& a, int lane, Deal& deal) {
+  int sum = 0, most = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int n = b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
+    sum += n;
+    most = max(most, n);
+  }
+  deal.total = __reduce_add_sync(0xffffffffu, sum) * a.nkv;
+  most = __reduce_max_sync(0xffffffffu, most);
+  Share s = {0, 0, 0, 0};
+  const int blocks = (int)gridDim.x, me = (int)blockIdx.x;
+  const bool uncut = (int64_t)a.B * a.nkv <= blocks && most <= deal.total / blocks + kCutCost;
+  deal.grid = uncut ? 0 : min(blocks, deal.total);
+  if (uncut ? me >= a.B * a.nkv : me >= deal.grid) return s;
+  if (!uncut) {
+    s.c0 = share_begin(deal, me);
+    s.c1 = share_begin(deal, me + 1);
+  }
+  // the sequence whose chunks hold c0 (uncut: sequence me / nkv)
+  const int want = uncut ? me / a.nkv : s.c0 / a.nkv;
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int n = b0 + lane < a.B ? chunk_count(a, b0 + lane) : 0;
@@ -175,11 +175,15 @@ __device__ __forceinline__ Share find_share(const Args& a, int lane, int& grid) 
       const int u = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += u;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > want);
+    const uint32_t hit = __ballot_sync(0xffffffffu, uncut ? b0 + lane == want : base + incl > want);
     if (hit) {
-      const int l = __ffs(hit) - 1;
+      const int l = __ffs(hit) - 1, mine = __shfl_sync(0xffffffffu, n, l);
       s.b = b0 + l;
       s.before = (base + __shfl_sync(0xffffffffu, incl - n, l)) * a.nkv;
+      if (uncut) {
+        s.c0 = s.before + (me % a.nkv) * mine;
+        s.c1 = s.c0 + mine;
+      }
       return s;
     }
     base += __shfl_sync(0xffffffffu, incl, 31);
@@ -211,100 +215,94 @@ __device__ __forceinline__ bool next_segment(const Args& a, Share& s, Segment& g
   return true;
 }
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_int4_kernel(const Args a) {
-  using L = DecLayout<HD, NT>;
-  constexpr int kG = L::kGroups, kQ = 8 * NT;
+template <int HD>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_int4_kernel(const Args a) {
+  using L = DecLayout<HD>;
+  constexpr int kG = L::kGroups;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* empty = full + L::kStages;
-  volatile uint32_t* bad_tiles = reinterpret_cast<uint32_t*>(empty + L::kStages);    // a bit per 16 keys of the stage
-  __shared__ int abort_flag;
-  __shared__ int merge_me;
+  __shared__ int abort_flag, merge_me;
   volatile int* abort_v = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < L::kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kWarps);
-    }
-    fence_barrier_init();
-  }
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * L::kStages;    // this warp's ring
+  uint8_t* ring = smem + warp * L::kStages * L::kStage;
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < L::kStages) mbar_init(&full[lane], 1);
+  fence_barrier_init();
   pdl_trigger();
   pdl_wait();
   __syncthreads();
-  int grid;
-  Share share = find_share(a, lane, grid);
-  Segment g;
+  Deal deal;
+  Share share = find_share(a, lane, deal);
 
-  if (warp == kWarps) {
-    // ---------------- producer ----------------
-    int it = 0;
-    int issued[L::kStages] = {};
-    bool ok = true;
-    while (ok && next_segment(a, share, g)) {
-      const int* table = a.tables + (int64_t)g.b * a.width;
-      for (int c = g.first; ok && c < g.first + g.n; ++c, ++it) {
-        const int s = it % L::kStages, u = it / L::kStages;
-        if (u >= 1) ok = __all_sync(0xffffffffu, wait_phase(&empty[s], (u - 1) & 1, abort_v, a.status, kTimeoutSmemEmpty));
-        if (!ok) break;
-        // lane i takes the i-th page that the chunk touches; runs are whole 16-key tiles of a page
-        const int k0 = c * kChunk, kend = min(k0 + kChunk, (g.keys + 15) & ~15);
-        const int page = k0 / a.bs + lane;
-        const int from = max(k0, page * a.bs), to = min(kend, (page + 1) * a.bs);
-        const bool mine = lane < kChunk / 16 + 1 && from < to;
-        int blk = 0;
-        bool bad = false;
-        if (mine) {
-          blk = table[page];
-          bad = blk < 0 || blk >= a.nblk;
-          if (bad) record_error(a.status, kBadIndex);
-        }
-        uint32_t flags = 0;
-        if (bad) flags = ((1u << ((to - k0) / 16)) - 1u) & ~((1u << ((from - k0) / 16)) - 1u);
-        flags = __reduce_or_sync(0xffffffffu, flags);
-        const int keys = mine && !bad ? to - from : 0;
-        const int total = __reduce_add_sync(0xffffffffu, keys);
-        if (lane == 0) {
-          bad_tiles[s] = flags;                    // published by the arrival below
-          mbar_expect_tx(&full[s], (uint32_t)total * (HD + 4 * kG));
-        }
-        __syncwarp();
-        if (keys > 0) {
-          const size_t row = ((size_t)blk * a.nkv + g.h) * a.bs + (from - page * a.bs);
-          const uint32_t st = smem_u32(smem) + s * L::kStage;
-          const int at = from - k0;
-          bulk_copy(st + at * (HD / 2), a.kp.codes + row * (HD / 2), keys * (HD / 2), &full[s]);
-          bulk_copy(st + 2 * L::kCodes + at * 2 * kG, a.kp.words + row * kG, keys * 2 * kG, &full[s]);
-          bulk_copy(st + L::kCodes + at * (HD / 2), a.vp.codes + row * (HD / 2), keys * (HD / 2), &full[s]);
-          bulk_copy(st + 2 * L::kCodes + L::kWords + at * 2 * kG, a.vp.words + row * kG, keys * 2 * kG, &full[s]);
-        }
-        issued[s] = u + 1;
-      }
+  // ---- copies: this warp's 32 keys of the chunks of the share, kStages of them ahead ----
+  Share ahead = share;
+  Segment pg;
+  int left = 0, chunk = 0, blk = 0, first_row = 0, issued = 0;    // chunks left of the segment, the next one, its block
+  uint32_t gone = 0;                                       // two bits a stage: 16-key tiles that are not there
+  bool more = true;
+  // Lanes 0..7: two pages (32 keys never touch more, pages hold whole 16-key tiles) x four tensors: codes of
+  // K and V, words of K and V.
+  const int tensor = lane >> 1 & 3, per_key = tensor < 2 ? HD / 2 : 2 * kG;
+  const uint8_t* source = tensor == 0 ? a.kp.codes : tensor == 1 ? a.vp.codes
+                          : reinterpret_cast<const uint8_t*>(tensor == 2 ? a.kp.words : a.vp.words);
+  const uint32_t dest = smem_u32(ring) + (tensor < 2 ? tensor * L::kCodes : 2 * L::kCodes + (tensor & 1) * L::kWords);
+  int from = 0, to = 0;                                    // keys of this lane's page in the next chunk, from its k0 on
+  auto find_next = [&]() {
+    if (left > 0) ++chunk;
+    else if ((more = next_segment(a, ahead, pg))) chunk = pg.first, left = pg.n;
+    if (!more) return;
+    --left;
+    const int k0 = chunk * kChunk + warp * kWarpKeys;
+    const int page = (int)(a.page_magic ? __umulhi((uint32_t)k0 / 16u, a.page_magic) : (uint32_t)k0 / 16u) + (lane & 1);
+    from = max(0, page * a.bs - k0);
+    to = min(min(kWarpKeys, (page + 1) * a.bs - k0), ((pg.keys + 15) & ~15) - k0);
+    if (lane >= 8) to = 0;
+    blk = from < to ? __ldg(a.tables + (int64_t)pg.b * a.width + page) : 0;
+    first_row = k0 + from - page * a.bs;
+  };
+  auto issue = [&]() {
+    if (!more) return;
+    const int s = issued % L::kStages;
+    bool mine = from < to;
+    const bool bad = mine && (uint32_t)blk >= (uint32_t)a.nblk;
+    int total = max(0, min(kWarpKeys, ((pg.keys + 15) & ~15) - (chunk * kChunk + warp * kWarpKeys)));
+    gone &= ~(3u << (2 * s));
+    if (__any_sync(0xffffffffu, bad)) {
+      if (bad) record_error(a.status, kBadIndex);
+      const uint32_t flags = bad ? ((1u << (to / 16)) - 1u) & ~((1u << (from / 16)) - 1u) : 0u;
+      gone |= __reduce_or_sync(0xffffffffu, flags) << (2 * s);
+      total -= 16 * __popc(gone >> (2 * s) & 3u);
+      mine = mine && !bad;
     }
-    // every copy has landed before the block may end
-    for (int s = 0; s < L::kStages; ++s)
-      if (issued[s] > 0) mbar_wait(&full[s], (issued[s] - 1) & 1);
-    return;
-  }
+    if (lane == 0) mbar_expect_tx(&full[s], (uint32_t)total * (HD + 4 * kG));
+    __syncwarp();
+    if (mine) {
+      const int64_t row = ((int64_t)blk * a.nkv + pg.h) * a.bs + first_row;
+      bulk_copy(dest + s * L::kStage + from * per_key, source + row * per_key, (to - from) * per_key, &full[s]);
+    }
+    ++issued;
+    find_next();
+  };
+  find_next();
+#pragma unroll 1
+  for (int i = 0; i < L::kStages; ++i) issue();
 
-  // ---------------- consumers ----------------
   const int gid = lane >> 2, t4 = lane & 3;
   const int group_heads = a.nh / a.nkv;
-  const int row0 = blockIdx.y * kQ, rows = min(kQ, a.nq * group_heads - row0);
+  const int row0 = blockIdx.y * kRows, rows = min(kRows, a.nq * group_heads - row0);
   float* merge = reinterpret_cast<float*>(smem + L::kMergeOff);
   float2* ml = reinterpret_cast<float2*>(smem + L::kMlOff);
 
   // sequences without keys: zeros
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
     if (key_count(a, b) == 0)
-      for (int i = threadIdx.x; i < a.nkv * rows * (HD / 8); i += kWarps * 32) {
+      for (int i = threadIdx.x; i < a.nkv * rows * (HD / 8); i += kThreads) {
         const int r = i / (HD / 8) % rows + row0, h = i / (HD / 8) / rows;
         const size_t at = ((size_t)b * a.nq + r / group_heads) * a.nh + h * group_heads + r % group_heads;
         *reinterpret_cast<uint4*>(a.out + at * HD + (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
       }
 
+  Segment g;
   int it = 0;
   bool ok = true;
   while (next_segment(a, share, g)) {
@@ -313,84 +311,44 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
       r += row0;
       return ((size_t)g.b * a.nq + r / group_heads) * a.nh + g.h * group_heads + r % group_heads;
     };
-    // Q^T operand: row gid of each 8-row tile as fp16 after scaling it by a power of two to a largest value
-    // in [2^14, 2^15); for group g and word i the dims 64 g + 16 t4 + 8 i + (s, s + 4)
-    uint32_t qf[NT][kG][2][4];
-    float back[NT][2];                             // rows 2 t4, 2 t4 + 1: what a score is multiplied by
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool live = n * 8 + gid < rows;
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + row_of(live ? n * 8 + gid : 0) * HD);
-      uint4 v[kG][2];
-      uint32_t most = 0;                           // bit pattern of the largest magnitude
+    // Q^T operand: row gid; for group g and word i the dims 64 g + 16 t4 + 8 i + (s, s + 4), times 4 for even s and
+    // 1/4 for odd s: with the codes' /64 and /4 every product is a sixteenth
+    uint32_t qf[kG][2][4];
+    {
+      const bool live = gid < rows;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + row_of(live ? gid : 0) * HD);
 #pragma unroll
       for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          v[gr][i] = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {v[gr][i].x, v[gr][i].y, v[gr][i].z, v[gr][i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) most = max(most, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+          const uint4 v = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
+          qf[gr][i][0] = mul_bf16x2(__byte_perm(v.x, v.z, 0x5410), 0x40804080u);
+          qf[gr][i][1] = mul_bf16x2(__byte_perm(v.x, v.z, 0x7632), 0x3e803e80u);
+          qf[gr][i][2] = mul_bf16x2(__byte_perm(v.y, v.w, 0x5410), 0x40804080u);
+          qf[gr][i][3] = mul_bf16x2(__byte_perm(v.y, v.w, 0x7632), 0x3e803e80u);
         }
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // 2^k in two factors, k = 14 - exponent (subnormals count as 2^-126)
-      const int k = 14 + 127 - max(1, (int)(most >> 7)), k0 = k >> 1, k1 = k - k0;
-      const float up0 = __uint_as_float((uint32_t)(127 + k0) << 23), up1 = __uint_as_float((uint32_t)(127 + k1) << 23);
-#pragma unroll
-      for (int gr = 0; gr < kG; ++gr)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t w[4] = {v[gr][i].x, v[gr][i].y, v[gr][i].z, v[gr][i].w};
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[2 * e] = __uint_as_float(w[e] << 16) * up0 * up1;
-            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u) * up0 * up1;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[n][gr][i][e] = pack2_f16(x[e], x[e + 4]);
-        }
-      // an infinity or NaN in the row: NaN scores
-      const float down = most >= 0x7f80u ? __uint_as_float(0x7fc00000u)
-                                         : __uint_as_float((uint32_t)(127 - k0) << 23) * a.scale_log2 *
-                                               __uint_as_float((uint32_t)(127 - k1) << 23);
-      back[n][0] = __shfl_sync(0xffffffffu, down, t4 * 8);
-      back[n][1] = __shfl_sync(0xffffffffu, down, t4 * 8 + 4);
     }
-    // keys that row r of the block sees
+    // keys that row r of the block sees, and keys that all its rows see
     auto limit = [&](int r) { return r < rows ? min(g.keys, a.lens[g.b] - a.nq + (row0 + r) / group_heads + 1) : 0; };
-    // keys below this are seen by every row of the tile
     const int all_see = min(g.keys, a.lens[g.b] - a.nq + row0 / group_heads + 1);
 
-    float o[NT][kG][4][4];
     // m: the reference that exponents are taken from, top: the score that moves it (-inf: none seen yet)
-    float m[NT][2], top[NT][2], l[NT][2];
+    float o[kG][4][4], m[2] = {0.f, 0.f}, top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
-      for (int gr = 0; gr < kG; ++gr)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][gr][j][e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[n][e] = 0.f;
-        top[n][e] = -INFINITY;
-        l[n][e] = 0.f;
-      }
-    }
+        for (int e = 0; e < 4; ++e) o[gr][j][e] = 0.f;
 
     for (int c = g.first; c < g.first + g.n; ++c, ++it) {
       const int s = it % L::kStages;
       ok = ok && __all_sync(0xffffffffu, wait_phase(&full[s], (it / L::kStages) & 1, abort_v, a.status, kTimeoutTmaFull));
       if (!ok) break;
-      const uint8_t* st = smem + s * L::kStage;
-      const uint32_t bad = bad_tiles[s];
+      const uint8_t* st = ring + s * L::kStage;
       // 16 keys; edge: some row of this block does not see some of them
       auto tile = [&](auto edge, int at) {
-        const int k0 = c * kChunk + at;
+        const int k0 = c * kChunk + warp * kWarpKeys + at;
         // Row m of the tile is key (m & 8) + ((m & 7) >> 1) + 4 (m & 1): the four rows that the four lanes
         // of a group read together for V then lie in two bank halves instead of one.
         const int key_a = (gid >> 1) + 4 * (gid & 1), key_b = key_a + 8;
@@ -405,76 +363,57 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
         auto scale = [](uint32_t w, int gr) { return __uint_as_float((gr == 0 ? w << 16 : w) & 0x7ff00000u); };
         const uint32_t kwa = words(kw, at + key_a), kwb = words(kw, at + key_b);
         const uint32_t vwa = words(vw, at + key_a), vwb = words(vw, at + key_b);
-        float p[NT][4];                            // [key a row 0, key a row 1, key b row 0, key b row 1]
+        float p[4];                                // [key a row 0, key a row 1, key b row 0, key b row 1]
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
           const uint2 wa = *reinterpret_cast<const uint2*>(ka + gr * 32);
           const uint2 wb = *reinterpret_cast<const uint2*>(ka + gr * 32 + 8 * (HD / 2));
-          // -(1024 + z) of each key, twice, and -(64 + z)
-          const uint32_t za = mask_or(__byte_perm(kwa, 0, gr ? 0x3232 : 0x1010), 0x000f000fu, 0xe400e400u);
-          const uint32_t zb = mask_or(__byte_perm(kwb, 0, gr ? 0x3232 : 0x1010), 0x000f000fu, 0xe400e400u);
-          const uint32_t za64 = add_f16x2(za, 0x63806380u), zb64 = add_f16x2(zb, 0x63806380u);
-          float sacc[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sacc[n][e] = 0.f;
+          const Zeros za = zeros(__byte_perm(kwa, 0, gr ? 0x3232 : 0x1010)), zb = zeros(__byte_perm(kwb, 0, gr ? 0x3232 : 0x1010));
+          float sacc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             uint32_t ya[4], yb[4];
-            codes_f16(i ? wa.y : wa.x, za, za64, ya);
-            codes_f16(i ? wb.y : wb.x, zb, zb64, yb);
+            codes_bf16(i ? wa.y : wa.x, za, ya);
+            codes_bf16(i ? wb.y : wb.x, zb, yb);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; e += 2)
-                mma_f16(sacc[n], ya[e], yb[e], ya[e + 1], yb[e + 1], qf[n][gr][i][e], qf[n][gr][i][e + 1]);
+            for (int e = 0; e < 4; e += 2)
+              mma_bf16(sacc, ya[e], yb[e], ya[e + 1], yb[e + 1], qf[gr][i][e], qf[gr][i][e + 1]);
           }
           const float ska = scale(kwa, gr), skb = scale(kwb, gr);
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[n][e] = fmaf(e < 2 ? ska : skb, sacc[n][e], gr == 0 ? 0.f : p[n][e]);
+          for (int e = 0; e < 4; ++e) p[e] = gr == 0 ? (e < 2 ? ska : skb) * sacc[e] : fmaf(e < 2 ? ska : skb, sacc[e], p[e]);
         }
         bool grow = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = p[n][e] * back[n][e & 1];
-            if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(n * 8 + t4 * 2 + (e & 1))) x = -INFINITY;
-            p[n][e] = x;
-            grow |= x > top[n][e & 1];
-          }
+        for (int e = 0; e < 4; ++e) {
+          p[e] *= a.scale_log2;
+          if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(t4 * 2 + (e & 1))) p[e] = -INFINITY;
+          grow |= p[e] > top[e & 1];
+        }
         // the reference maximum moves only when a score passes it by 2^8 (first tile: from -inf)
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(p[e], p[e + 2]);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(p[n][e], p[n][e + 2]);
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            // f = 2^(old - new); a row that has seen no key keeps reference 0 and the next score moves it
+            const bool none = top[e] == -INFINITY;
+            const float mn = none ? mx : fmaxf(m[e], mx), f = none ? 0.f : umma::ex2(m[e] - mn);
+            m[e] = mn == -INFINITY ? 0.f : mn;
+            top[e] = mn + kRescaleLog2;
+            l[e] *= f;
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-              // f = 2^(old - new); a row that has seen no key keeps reference 0 and the next score moves it
-              const bool none = top[n][e] == -INFINITY;
-              const float mn = none ? mx : fmaxf(m[n][e], mx), f = none ? 0.f : umma::ex2(m[n][e] - mn);
-              m[n][e] = mn == -INFINITY ? 0.f : mn;
-              top[n][e] = mn + kRescaleLog2;
-              l[n][e] *= f;
+            for (int gr = 0; gr < kG; ++gr)
 #pragma unroll
-              for (int gr = 0; gr < kG; ++gr) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][gr][j][e] *= f, o[n][gr][j][e + 2] *= f;
-              }
-            }
+              for (int j = 0; j < 4; ++j) o[gr][j][e] *= f, o[gr][j][e + 2] *= f;
+          }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[n][e] = umma::ex2(p[n][e] - m[n][e & 1]);
-            l[n][e & 1] += p[n][e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          p[e] = umma::ex2(p[e] - m[e & 1]);
+          l[e & 1] += p[e];
+        }
         // O^T: words of keys (rows 2 t4, 2 t4 + 1, + 8) for dims 64 g + 8 gid ..; row 2 t4 is key t4, row
         // 2 t4 + 1 key t4 + 4
         const uint8_t* v0 = st + L::kCodes + (at + t4) * (HD / 2) + gid * 4;
@@ -482,80 +421,70 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
                        z9 = words(vw, at + t4 + 12);
 #pragma unroll
         for (int gr = 0; gr < kG; ++gr) {
-          uint32_t w0[NT], w1[NT];
+          float w[4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              w[e] = p[n][e] * scale(e < 2 ? vwa : vwb, gr);
-              // a key that this row does not see may hold anything, NaN scales among it
-              if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(n * 8 + t4 * 2 + (e & 1))) w[e] = 0.f;
-            }
-            const uint32_t lo = umma::pack2_bf16(w[0], w[1]), hi = umma::pack2_bf16(w[2], w[3]);
-            w0[n] = transpose8x8(lo);
-            w1[n] = transpose8x8(hi);
+          for (int e = 0; e < 4; ++e) {
+            w[e] = p[e] * scale(e < 2 ? vwa : vwb, gr);
+            // a key that this row does not see may hold anything, NaN scales among it
+            if (edge.value && k0 + (e < 2 ? key_a : key_b) >= limit(t4 * 2 + (e & 1))) w[e] = 0.f;
           }
+          const uint32_t w0 = transpose8x8(umma::pack2_bf16(w[0], w[1])), w1 = transpose8x8(umma::pack2_bf16(w[2], w[3]));
           const uint32_t x0 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32),
                          x1 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 4 * (HD / 2)),
                          x8 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 8 * (HD / 2)),
                          x9 = *reinterpret_cast<const uint32_t*>(v0 + gr * 32 + 12 * (HD / 2));
-          // 128 + z of the two keys of each pair
-          const uint32_t z01 = mask_or(__byte_perm(z0, z1, gr ? 0x7632 : 0x5410), 0x000f000fu, 0x43004300u);
-          const uint32_t z89 = mask_or(__byte_perm(z8, z9, gr ? 0x7632 : 0x5410), 0x000f000fu, 0x43004300u);
-          const uint32_t lo01 = __byte_perm(x0, x1, 0x5410), hi01 = __byte_perm(x0, x1, 0x7632);
-          const uint32_t lo89 = __byte_perm(x8, x9, 0x5410), hi89 = __byte_perm(x8, x9, 0x7632);
+          const Zeros z01 = zeros(__byte_perm(z0, z1, gr ? 0x7632 : 0x5410)), z89 = zeros(__byte_perm(z8, z9, gr ? 0x7632 : 0x5410));
+          uint32_t a0[4], a1[4], a2[4], a3[4];
+          codes_bf16(__byte_perm(x0, x1, 0x5410), z01, a0);
+          codes_bf16(__byte_perm(x0, x1, 0x7632), z01, a1);
+          codes_bf16(__byte_perm(x8, x9, 0x5410), z89, a2);
+          codes_bf16(__byte_perm(x8, x9, 0x7632), z89, a3);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a0 = sub_bf16x2(nibbles(lo01, j), z01), a1 = sub_bf16x2(nibbles(hi01, j), z01),
-                           a2 = sub_bf16x2(nibbles(lo89, j), z89), a3 = sub_bf16x2(nibbles(hi89, j), z89);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16(o[n][gr][j], a0, a1, a2, a3, w0[n], w1[n]);
-          }
+          for (int j = 0; j < 4; ++j) mma_bf16(o[gr][j], a0[j], a1[j], a2[j], a3[j], w0, w1);
         }
       };
-      const int at0 = warp * kWarpKeys, k0 = c * kChunk + at0;
-      if (k0 + kWarpKeys <= all_see && bad == 0u) {
+      const int k0 = c * kChunk + warp * kWarpKeys;
+      const uint32_t away = gone >> (2 * s) & 3u;
+      if (k0 + kWarpKeys <= all_see && away == 0u) {
 #pragma unroll
-        for (int i = 0; i < kWarpKeys; i += 16) tile(std::false_type(), at0 + i);
+        for (int i = 0; i < kWarpKeys; i += 16) tile(std::false_type(), i);
       } else {
 #pragma unroll 1
         for (int i = 0; i < kWarpKeys; i += 16)
-          if (k0 + i < g.keys && !((bad >> ((at0 + i) / 16)) & 1u)) tile(std::true_type(), at0 + i);
+          if (k0 + i < g.keys && !(away >> (i / 16) & 1u)) tile(std::true_type(), i);
       }
-      __syncwarp();
-      if (lane == 0) umma::mbar_arrive(&empty[s]);
+      __syncwarp();                                // every lane has read the stage
+      issue();
     }
 
     // ---- the warps' results of this segment meet in shared memory ----
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const int r = t4 * 2 + e;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = n * 8 + t4 * 2 + e;
+      for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+      if (gid == 0) ml[warp * kRows + r] = make_float2(top[e] - kRescaleLog2, l[e]);
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-        if (gid == 0) ml[warp * kQ + r] = make_float2(top[n][e] - kRescaleLog2, l[n][e]);
-#pragma unroll
-        for (int gr = 0; gr < kG; ++gr) {
-          float* dst = merge + (warp * kQ + r) * L::kRow + gr * 64 + gid * 8;
-          *reinterpret_cast<float4*>(dst) = make_float4(o[n][gr][0][e], o[n][gr][1][e], o[n][gr][2][e], o[n][gr][3][e]);
-          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[n][gr][0][e + 2], o[n][gr][1][e + 2], o[n][gr][2][e + 2], o[n][gr][3][e + 2]);
-        }
+      for (int gr = 0; gr < kG; ++gr) {
+        float* dst = merge + (warp * kRows + r) * L::kRow + gr * 64 + gid * 8;
+        *reinterpret_cast<float4*>(dst) = make_float4(o[gr][0][e] * 64.f, o[gr][1][e] * 4.f, o[gr][2][e] * 64.f, o[gr][3][e] * 4.f);
+        *reinterpret_cast<float4*>(dst + 4) = 
+            make_float4(o[gr][0][e + 2] * 64.f, o[gr][1][e + 2] * 4.f, o[gr][2][e + 2] * 64.f, o[gr][3][e + 2] * 4.f);
       }
-    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    }
+    __syncthreads();
     const bool whole = g.n == g.chunks;
-    for (int i = threadIdx.x; i < rows * (HD / 8); i += kWarps * 32) {
+    for (int i = threadIdx.x; i < rows * (HD / 8); i += kThreads) {
       const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
       float mx = -INFINITY, sum = 0.f, acc[8] = {};
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * kQ + r].x);
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * kRows + r].x);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 x = ml[w * kQ + r];
+        const float2 x = ml[w * kRows + r];
         const float f = x.x == -INFINITY ? 0.f : umma::ex2(x.x - mx);
         sum += f * x.y;
-        const float* src = merge + (w * kQ + r) * L::kRow + d;
+        const float* src = merge + (w * kRows + r) * L::kRow + d;
         if (f != 0.f)
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] += f * src[e];
@@ -576,32 +505,33 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
     }
     if (!whole) {
       // pieces of this pair: cut where the shares of the blocks begin
-      const int i0 = (int)(((int64_t)(g.pair0 + 1) * grid - 1) / share.total);
-      const int i1 = (int)(((int64_t)(g.pair0 + g.chunks) * grid - 1) / share.total);
+      const int i0 = (int)(((int64_t)(g.pair0 + 1) * deal.grid - 1) / deal.total);
+      const int i1 = (int)(((int64_t)(g.pair0 + g.chunks) * deal.grid - 1) / deal.total);
       const int pieces = i1 - i0 + 1;
       __threadfence();
-      asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+      __syncthreads();
       if (threadIdx.x == 0)
         merge_me = atomicInc(reinterpret_cast<unsigned*>(a.counters) + ((size_t)g.b * a.nkv + g.h) * a.row_tiles + blockIdx.y,
                              (unsigned)pieces - 1u) == (unsigned)pieces - 1u;
-      asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+      __syncthreads();
       if (merge_me) {
         __threadfence();
-        for (int i = threadIdx.x; i < rows * (HD / 8); i += kWarps * 32) {
+        for (int i = threadIdx.x; i < rows * (HD / 8); i += kThreads) {
           const int r = i / (HD / 8), d = (i % (HD / 8)) * 8;
           const size_t row = row_of(r);
           float mx = -INFINITY, sum = 0.f, acc[8] = {};
+#pragma unroll 4
           for (int x = 0; x < pieces; ++x) {
-            const int first = max(0, share_begin(share.total, grid, i0 + x) - g.pair0);
+            const int first = max(0, share_begin(deal, i0 + x) - g.pair0);
             const size_t slot = row * a.max_splits + first;
             const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot);
+            const float4* src = reinterpret_cast<const float4*>(a.part_o + slot * HD + d);
+            const float4 y0 = __ldcg(src), y1 = __ldcg(src + 1);
+            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
             if (v.y == 0.f) continue;              // saw no key
             const float mn = fmaxf(mx, v.x), f = mx == -INFINITY ? 0.f : umma::ex2(mx - mn), fx = umma::ex2(v.x - mn);
             mx = mn;
             sum = sum * f + fx * v.y;
-            const float4* src = reinterpret_cast<const float4*>(a.part_o + slot * HD + d);
-            const float4 y0 = __ldcg(src), y1 = __ldcg(src + 1);
-            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f + fx * y[e];
           }
@@ -612,8 +542,10 @@ __global__ void __launch_bounds__(kThreads, DecLayout<HD, NT>::kBlocks) decode_i
         }
       }
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");    // the merge rows are free again
+    __syncthreads();                               // the merge rows are free again
   }
+  // after a wait ran out: the copies in flight have landed before the block may end
+  for (; it < issued; ++it) mbar_wait(&full[it % L::kStages], (it / L::kStages) & 1);
 }
 
 }  // namespace
@@ -644,31 +576,26 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
                      counters.device() == dev && max_splits * kChunk >= cap && part_o.numel() >= T * nh * max_splits * hd &&
                      part_ml.numel() >= T * nh * max_splits * 2 && counters.numel() >= T * nh,
                  "decode workspace too small for this batch");
+  // a page is tile * magic >> 32: exact while tile * (bs / 16) stays below 2^32
+  LSB_INT4_CHECK((cap / 16 + 8) * (bs / 16) < (1ll << 32) || ((bs / 16) & (bs / 16 - 1)) == 0, "context too long for this block size");
   LSB_INT4_CHECK(B * nkv * ((cap + kChunk - 1) / kChunk) < INT32_MAX, "more 128-key chunks than an int32 can count");
-  LSB_INT4_CHECK(T * nh < INT32_MAX && nq * (nh / nkv) <= 16 * 65535, "batch exceeds int32 rows");
+  LSB_INT4_CHECK(T * nh < INT32_MAX && nq * (nh / nkv) <= kRows * 65535, "batch exceeds int32 rows");
   const at::cuda::CUDAGuard guard(dev);
-  const int rows = (int)(nq * (nh / nkv)), nt = rows > 8 ? 2 : 1, tiles = (rows + 8 * nt - 1) / (8 * nt);
+  const int tiles = (int)((nq * (nh / nkv) + kRows - 1) / kRows);
   Args a = {(bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), {kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
             {vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, lens.data_ptr<int>(), tables.data_ptr<int>(),
             part_o.data_ptr<float>(), part_ml.data_ptr<float>(), counters.data_ptr<int>(), status_ptr(status),
-            (float)(scale * 1.4426950408889634), (int)tables.size(1), (int)B, (int)nq, (int)nh, (int)nkv, (int)bs,
-            (int)kc.size(0), (int)max_splits, tiles};
-  auto go = [&](auto kern, int smem, int per_sm) {
+            (float)(scale * 16 * 1.4426950408889634), (int)tables.size(1), (int)B, (int)nq, (int)nh, (int)nkv, (int)bs,
+            (int)kc.size(0), (int)max_splits, tiles, bs == 16 ? 0u : (uint32_t)(((1ll << 32) + bs / 16 - 1) / (bs / 16))};
+  auto go = [&](auto kern, int smem) {
     ensure_dynamic_smem((const void*)kern, smem);
     // as many blocks as fit the GPU at once, shared by the row tiles, and no more than there can be chunks
     const int64_t most = B * nkv * std::max<int64_t>(1, (cap + kChunk - 1) / kChunk);
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(most, 148 * per_sm / tiles));
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(most, 148 * kBlocksPerSm / tiles));
     launch_pdl(kern, dim3((unsigned)grid, tiles), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(), a);
   };
-#define LSB_DEC(HD, NT) go(decode_int4_kernel<HD, NT>, DecLayout<HD, NT>::kBytes, DecLayout<HD, NT>::kBlocks)
-  if (hd == 128) {
-    if (nt == 1) LSB_DEC(128, 1);
-    else LSB_DEC(128, 2);
-  } else {
-    if (nt == 1) LSB_DEC(64, 1);
-    else LSB_DEC(64, 2);
-  }
-#undef LSB_DEC
+  if (hd == 128) go(decode_int4_kernel<128>, DecLayout<128>::kBytes);
+  else go(decode_int4_kernel<64>, DecLayout<64>::kBytes);
   const cudaError_t e = cudaGetLastError();
   LSB_INT4_CHECK(e == cudaSuccess, std::string("decode_attention_int4 launch failed: ") + cudaGetErrorString(e));
 }
