@@ -237,7 +237,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_int4_kernel(con
   // ---- copies: this warp's 32 keys of the chunks of the share, kStages of them ahead ----
   Share ahead = share;
   Segment pg;
-  int left = 0, chunk = 0, blk = 0, first_row = 0, issued = 0;    // chunks left of the segment, the next one, its block
+  // chunks left of the segment; first key and keys there for the next one; a lane's block and row in it
+  int left = 0, k_next = 0, there = 0, k_end = 0, blk = 0, first_row = 0, issued = 0;
   uint32_t gone = 0;                                       // two bits a stage: 16-key tiles that are not there
   bool more = true;
   // Lanes 0..7: two pages (32 keys never touch more, pages hold whole 16-key tiles) x four tensors: codes of
@@ -246,27 +247,32 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_int4_kernel(con
   const uint8_t* source = tensor == 0 ? a.kp.codes : tensor == 1 ? a.vp.codes
                           : reinterpret_cast<const uint8_t*>(tensor == 2 ? a.kp.words : a.vp.words);
   const uint32_t dest = smem_u32(ring) + (tensor < 2 ? tensor * L::kCodes : 2 * L::kCodes + (tensor & 1) * L::kWords);
-  int from = 0, to = 0;                                    // keys of this lane's page in the next chunk, from its k0 on
+  const int cap = lane < 8 ? kWarpKeys : 0;
+  int from = 0, to = 0;                                    // keys of this lane's page in the next chunk
   auto find_next = [&]() {
-    if (left > 0) ++chunk;
-    else if ((more = next_segment(a, ahead, pg))) chunk = pg.first, left = pg.n;
-    if (!more) return;
-    --left;
-    const int k0 = chunk * kChunk + warp * kWarpKeys;
-    const int page = (int)(a.page_magic ? __umulhi((uint32_t)k0 / 16u, a.page_magic) : (uint32_t)k0 / 16u) + (lane & 1);
-    from = max(0, page * a.bs - k0);
-    to = min(min(kWarpKeys, (page + 1) * a.bs - k0), ((pg.keys + 15) & ~15) - k0);
-    if (lane >= 8) to = 0;
-    blk = from < to ? __ldg(a.tables + (int64_t)pg.b * a.width + page) : 0;
-    first_row = k0 + from - page * a.bs;
+    k_next += kChunk;
+    if (--left < 0) {
+      more = next_segment(a, ahead, pg);
+      if (!more) return;
+      left = pg.n - 1;
+      k_next = pg.first * kChunk + warp * kWarpKeys;
+      k_end = (pg.keys + 15) & ~15;
+    }
+    there = max(0, min(kWarpKeys, k_end - k_next));
+    const uint32_t tile = (uint32_t)k_next / 16u;
+    const int page = (int)(a.page_magic ? __umulhi(tile, a.page_magic) : tile) + (lane & 1), start = page * a.bs - k_next;
+    from = max(0, start);
+    to = min(min(cap, there), start + a.bs);
+    first_row = from - start;
+    if (from < to) blk = __ldg(a.tables + (int64_t)pg.b * a.width + page);
   };
   auto issue = [&]() {
     if (!more) return;
     const int s = issued % L::kStages;
     bool mine = from < to;
     const bool bad = mine && (uint32_t)blk >= (uint32_t)a.nblk;
-    int total = max(0, min(kWarpKeys, ((pg.keys + 15) & ~15) - (chunk * kChunk + warp * kWarpKeys)));
-    gone &= ~(3u << (2 * s));
+    int total = there;
+    if (gone) gone &= ~(3u << (2 * s));
     if (__any_sync(0xffffffffu, bad)) {
       if (bad) record_error(a.status, kBadIndex);
       const uint32_t flags = bad ? ((1u << (to / 16)) - 1u) & ~((1u << (from / 16)) - 1u) : 0u;

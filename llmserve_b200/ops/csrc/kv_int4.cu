@@ -39,9 +39,16 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 //
 // x / s is x * (1 / s): for bf16 inputs (kSnap) a quotient that lies exactly half way between two
 // codes must stay there.  x has eight significant bits and s four, so a quotient above 1/4 that is
-// not half way is at least 2^-6 / 30 = 5.2e-4 away from it; rounding to a multiple of 2^-13 (adding
-// and subtracting 1536) moves it by 6.1e-5 at most and removes the 2e-6 that the reciprocal can add,
-// which gives the division's result for a third of its instructions.
+// not half way is at least 2^-6 / 30 = 5.2e-4 away from it; rounding to a multiple of 2^-13 (the sum with
+// 1536) moves it by 6.1e-5 at most and removes the 4e-6 that an approximate reciprocal adds, which gives
+// the division's result.  The sum with 1.5 * 2^23 then rounds to the integer, half to even, and leaves it
+// in the low mantissa bits: no conversion instruction (a quarter of the rate) and no division (16384 rows
+// of 8 heads of 128, store and read-back: 73 us with them, 38 us without).
+template <bool kSnap>
+__device__ __forceinline__ int round_code(float x, float inv) {
+  const float y = kSnap ? __fadd_rn(fmaf(x, inv, 1536.f), 12582912.f - 1536.f) : fmaf(x, inv, 12582912.f);
+  return __float_as_int(y) - 0x4b400000;
+}
 template <bool kSnap>
 __device__ __forceinline__ uint32_t quantise8(const float* x, uint32_t& word) {
   float mx = 0.f, mn = 0.f;
@@ -55,7 +62,8 @@ __device__ __forceinline__ uint32_t quantise8(const float* x, uint32_t& word) {
     mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
   }
-  const float r = __fdiv_rn(0.5f * mx - 0.5f * mn, 7.5f);
+  // r = (range / 2) / 7.5: product with the reciprocal and one correction, exact where the quotient is
+  const float half = 0.5f * mx - 0.5f * mn, q = half * 0.13333334f, r = fmaf(fmaf(-q, 7.5f, half), 0.13333334f, q);
   if (!(r <= 3.402823466e38f)) {          // NaN or infinity in the group
     word = 0x7fc0u;
     return 0u;
@@ -63,15 +71,13 @@ __device__ __forceinline__ uint32_t quantise8(const float* x, uint32_t& word) {
   word = 0u;
   if (r < 1.17549435e-38f) return 0u;
   const uint32_t sbits = (__float_as_uint(r) + 0xfffffu) & 0x7ff00000u;
-  const float s = __uint_as_float(sbits), inv = __fdiv_rn(1.f, s);
-  const int z = __float2int_rn(kSnap ? __fadd_rn(fmaf(-mn, inv, 1536.f), -1536.f) : -mn * inv);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__uint_as_float(sbits)));
+  const int z = round_code<kSnap>(-mn, inv);
   word = (sbits >> 16) | (uint32_t)z;
   uint32_t codes = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = __float2int_rn(kSnap ? __fadd_rn(fmaf(x[i], inv, 1536.f), -1536.f) : x[i] * inv) + z;
-    codes |= (uint32_t)min(c, 15) << (4 * i);
-  }
+  for (int i = 7; i >= 0; --i) codes = codes * 16u + (uint32_t)min(round_code<kSnap>(x[i], inv) + z, 15);
   return codes;
 }
 
@@ -82,6 +88,16 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* x) {
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
+}
+__device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -101,63 +117,68 @@ __device__ __forceinline__ bool page_row(int slot, int64_t num_slots, int nkv, i
   return true;
 }
 
-// grid.y: 0 = K, 1 = V.  Unit u of 8 dims: (token, head, part) in row-major order.
+// Unit u of 8 dims: (token, head, part) in row-major order; a lane takes it of K and of V, two independent
+// chains on one slot look-up.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) store_int4_kernel(
     const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t kst, int64_t ksh, int64_t vst, int64_t vsh,
     uint8_t* __restrict__ kc, int16_t* __restrict__ kw, uint8_t* __restrict__ vc, int16_t* __restrict__ vw,
-    const int* __restrict__ slots, int64_t units, int nkv, uint32_t bs, int64_t num_slots, int* status) {
+    const int* __restrict__ slots, uint32_t rows, uint32_t nkv, uint32_t bs, int64_t num_slots, int* status) {
   pdl_trigger();
   pdl_wait();
   constexpr int kLanes = HD / 8;
-  const bool is_v = blockIdx.y != 0;
-  const int64_t u0 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const bool live = u0 < units;
-  const int64_t u = live ? u0 : units - 1;         // tail lanes take part in the butterflies
-  const uint32_t lane = (uint32_t)u % kLanes;
-  const int64_t th = u / kLanes;
-  const int64_t t = th / nkv;
-  const int h = (int)(th - t * nkv);
-  const bf16* src = is_v ? v + t * vst + h * vsh : k + t * kst + h * ksh;
-  float x[8];
-  unpack_bf16x8(*reinterpret_cast<const uint4*>(src + lane * 8), x);
+  const uint32_t th0 = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const bool live = th0 < rows;
+  const uint32_t th = live ? th0 : rows - 1;       // tail lanes take part in the butterflies
+  const uint32_t t = th / nkv, h = th - t * nkv;
   const int slot = slots[t];
-  uint32_t word;
-  const uint32_t codes = quantise8<true>(x, word);
+  float x[8], y[8];
+  unpack_bf16x8(*reinterpret_cast<const uint4*>(k + t * kst + h * ksh + lane * 8), x);
+  unpack_bf16x8(*reinterpret_cast<const uint4*>(v + t * vst + h * vsh + lane * 8), y);
+  uint32_t word_k, word_v;
+  const uint32_t codes_k = quantise8<true>(x, word_k), codes_v = quantise8<true>(y, word_v);
   size_t row;
   if (!live || !page_row(slot, num_slots, nkv, h, bs, status, row)) return;
-  reinterpret_cast<uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane] = codes;
-  if (lane % 8 == 0) (is_v ? vw : kw)[row * (HD / kGroup) + lane / 8] = (int16_t)word;
+  reinterpret_cast<uint32_t*>(kc + row * (HD / 2))[lane] = codes_k;
+  reinterpret_cast<uint32_t*>(vc + row * (HD / 2))[lane] = codes_v;
+  if (lane % 8 == 0) {
+    kw[row * (HD / kGroup) + lane / 8] = (int16_t)word_k;
+    vw[row * (HD / kGroup) + lane / 8] = (int16_t)word_v;
+  }
+}
+
+// eight codes of one group as bf16.  128 + c is a bf16 with c in its low mantissa bits; pairs (n, n + 4) of
+// nibbles, put in order at the end
+__device__ __forceinline__ uint4 dequantise8(uint32_t c, uint32_t w) {
+  const uint32_t dup = __byte_perm(w, 0, 0x1010), s2 = dup & 0x7ff07ff0u, z2 = (dup & 0x000f000fu) | 0x43004300u;
+  uint32_t y[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) y[n] = mul2(sub2(((c >> (4 * n)) & 0x000f000fu) | 0x43004300u, z2), s2);
+  return make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                    __byte_perm(y[2], y[3], 0x7632));
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads) load_int4_kernel(
     bf16* __restrict__ k, bf16* __restrict__ v, const uint8_t* __restrict__ kc, const int16_t* __restrict__ kw,
-    const uint8_t* __restrict__ vc, const int16_t* __restrict__ vw, const int* __restrict__ slots, int64_t units,
-    int nkv, uint32_t bs, int64_t num_slots, int* status) {
+    const uint8_t* __restrict__ vc, const int16_t* __restrict__ vw, const int* __restrict__ slots, uint32_t rows,
+    uint32_t nkv, uint32_t bs, int64_t num_slots, int* status) {
   pdl_trigger();
   pdl_wait();
   constexpr int kLanes = HD / 8;
-  const bool is_v = blockIdx.y != 0;
-  const int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (u >= units) return;
-  const uint32_t lane = (uint32_t)u % kLanes;
-  const int64_t th = u / kLanes;
-  const int64_t t = th / nkv;
-  const int h = (int)(th - t * nkv);
-  uint4 o = make_uint4(0, 0, 0, 0);
+  const uint32_t th = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  if (th >= rows) return;
+  const uint32_t t = th / nkv, h = th - t * nkv;
+  uint32_t ck = 0, cv = 0, wk = 0, wv = 0;         // scale 0: zeros
   size_t row;
   if (page_row(slots[t], num_slots, nkv, h, bs, status, row)) {
-    const uint32_t c = reinterpret_cast<const uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane];
-    const uint32_t w = (uint16_t)(is_v ? vw : kw)[row * (HD / kGroup) + lane / 8];
-    const float s = word_scale(w);
-    const int z = (int)word_zero(w);
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = s * (float)((int)((c >> (4 * i)) & 15u) - z);
-    o = make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+    ck = reinterpret_cast<const uint32_t*>(kc + row * (HD / 2))[lane];
+    cv = reinterpret_cast<const uint32_t*>(vc + row * (HD / 2))[lane];
+    wk = (uint16_t)kw[row * (HD / kGroup) + lane / 8];
+    wv = (uint16_t)vw[row * (HD / kGroup) + lane / 8];
   }
-  *reinterpret_cast<uint4*>((is_v ? v : k) + u * 8) = o;
+  reinterpret_cast<uint4*>(k)[(size_t)th * kLanes + lane] = dequantise8(ck, wk);
+  reinterpret_cast<uint4*>(v)[(size_t)th * kLanes + lane] = dequantise8(cv, wv);
 }
 
 // One step's projection rows [T, (nh + 2 nkv) * HD] (bf16, or S fp32 split-K planes that are summed
@@ -174,16 +195,16 @@ __global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
   pdl_wait();
   constexpr int kLanes = HD / 8, kHalf = HD / 2;
   const int heads = nh + 2 * nkv;
-  const int64_t rows = (int64_t)T * heads;
-  const int64_t r0 = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const uint32_t rows = (uint32_t)T * heads;
+  const uint32_t r0 = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   const bool live = r0 < rows;
-  const int64_t r = live ? r0 : rows - 1;          // tail lanes take part in the butterflies
-  const int t = (int)(r / heads), head = (int)(r - (int64_t)t * heads);
+  const uint32_t r = live ? r0 : rows - 1;         // tail lanes take part in the butterflies
+  const int t = (int)(r / (uint32_t)heads), head = (int)(r - (uint32_t)t * heads);
   const int lane = threadIdx.x % kLanes, d0 = lane * 8;
   float x[8];
   if constexpr (kPlanes) {
-    const float* p = (const float*)qkv + r * HD + d0;
-    const int64_t plane = rows * HD;
+    const float* p = (const float*)qkv + (int64_t)r * HD + d0;
+    const int64_t plane = (int64_t)rows * HD;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
 #pragma unroll 4
@@ -194,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
       x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
     }
   } else {
-    unpack_bf16x8(*reinterpret_cast<const uint4*>((const bf16*)qkv + r * HD + d0), x);
+    unpack_bf16x8(*reinterpret_cast<const uint4*>((const bf16*)qkv + (int64_t)r * HD + d0), x);
   }
   const bool is_v = head >= nh + nkv;
   const bf16* w = head < nh ? q_w : k_w;
@@ -233,9 +254,17 @@ __global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + sign * y[i] * s[i];
   }
-  uint32_t word;
-  // values that are bf16 already (V of a bf16 projection) take the exact-tie form
-  const uint32_t codes = kPlanes ? quantise8<false>(x, word) : (is_v ? quantise8<true>(x, word) : quantise8<false>(x, word));
+  uint32_t word = 0, codes = 0;
+  if (__any_sync(0xffffffffu, head >= nh)) {       // a warp of query heads has nothing to quantise
+    // values that are bf16 already (V of a bf16 projection) take the exact-tie form
+    const bool all_v = !kPlanes && __all_sync(0xffffffffu, is_v), some_v = !kPlanes && __any_sync(0xffffffffu, is_v);
+    if (!all_v) codes = quantise8<false>(x, word);
+    if (some_v) {
+      uint32_t word_v;
+      const uint32_t codes_v = quantise8<true>(x, word_v);
+      if (is_v) codes = codes_v, word = word_v;
+    }
+  }
   if (!live) return;
   if (head < nh) {
     *reinterpret_cast<uint4*>(q_out + ((int64_t)t * nh + head) * HD + d0) =
@@ -276,18 +305,18 @@ void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw
   LSB_INT4_CHECK(k.size(1) == kc.size(1) && k.size(2) == kc.size(3) * 2, "k / v heads do not match the pages");
   check_int32(slots, "slot_mapping", 1, k.device());
   LSB_INT4_CHECK(slots.size(0) == k.size(0), "slot_mapping must hold one slot per token");
-  const int64_t units = k.numel() / 8;
-  if (units == 0) return;
-  LSB_INT4_CHECK(units / kThreads < INT32_MAX, "too many rows for one launch");
+  const int64_t rows = k.size(0) * k.size(1), per = kThreads / (k.size(2) / 8);
+  if (rows == 0) return;
+  LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
   const at::cuda::CUDAGuard g(k.device());
   k = rows_for_store(k);
   v = rows_for_store(v);
-  const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2);
+  const dim3 grid((unsigned)((rows + per - 1) / per));
   auto go = [&](auto kern) {
     launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (const bf16*)k.data_ptr(),
                (const bf16*)v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kc.data_ptr<uint8_t>(),
-               kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), slots.data_ptr<int>(), units,
-               (int)kc.size(1), (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
+               kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), slots.data_ptr<int>(),
+               (uint32_t)rows, (uint32_t)kc.size(1), (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
   };
   if (k.size(2) == 128) go(store_int4_kernel<128>);
   else go(store_int4_kernel<64>);
@@ -302,15 +331,15 @@ void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw,
                      k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.device() == k.device() &&
                      k.size(0) == slots.size(0) && k.size(1) == kc.size(1) && k.size(2) == kc.size(3) * 2,
                  "outputs must be contiguous bfloat16 [slots, kv_heads, head_dim]");
-  const int64_t units = k.numel() / 8;
-  if (units == 0) return;
-  LSB_INT4_CHECK(units / kThreads < INT32_MAX, "too many rows for one launch");
+  const int64_t rows = k.size(0) * k.size(1), per = kThreads / (k.size(2) / 8);
+  if (rows == 0) return;
+  LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
   const at::cuda::CUDAGuard g(k.device());
-  const dim3 grid((unsigned)((units + kThreads - 1) / kThreads), 2);
+  const dim3 grid((unsigned)((rows + per - 1) / per));
   auto go = [&](auto kern) {
     launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (bf16*)k.data_ptr(),
                (bf16*)v.data_ptr(), kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(),
-               vw.data_ptr<int16_t>(), slots.data_ptr<int>(), units, (int)kc.size(1), (uint32_t)kc.size(2),
+               vw.data_ptr<int16_t>(), slots.data_ptr<int>(), (uint32_t)rows, (uint32_t)kc.size(1), (uint32_t)kc.size(2),
                kc.size(0) * kc.size(2), status_ptr(status));
   };
   if (k.size(2) == 128) go(load_int4_kernel<128>);
@@ -349,7 +378,7 @@ void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::T
                    "norm weights must be contiguous bfloat16 [head_dim]");
   if (T == 0) return;
   const int64_t per = kThreads / (hd / 8), rows = T * (nh + 2 * nkv);
-  LSB_INT4_CHECK(T < INT32_MAX && rows / per < INT32_MAX, "too many rows for one launch");
+  LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
   const at::cuda::CUDAGuard g(dev);
   auto go = [&](auto kern) {
     launch_pdl(kern, dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(),
