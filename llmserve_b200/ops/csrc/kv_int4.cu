@@ -43,7 +43,7 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 // 1536) moves it by 6.1e-5 at most and removes the 4e-6 that an approximate reciprocal adds, which gives
 // the division's result.  The sum with 1.5 * 2^23 then rounds to the integer, half to even, and leaves it
 // in the low mantissa bits: no conversion instruction (a quarter of the rate) and no division (16384 rows
-// of 8 heads of 128, store and read-back: 73 us with them, 38 us without).
+// of 8 heads of 128, store and read-back: 73 us with them and 64-bit indexing, 43 us without).
 template <bool kSnap>
 __device__ __forceinline__ int round_code(float x, float inv) {
   const float y = kSnap ? __fadd_rn(fmaf(x, inv, 1536.f), 12582912.f - 1536.f) : fmaf(x, inv, 12582912.f);
@@ -184,99 +184,110 @@ __global__ void __launch_bounds__(kThreads) load_int4_kernel(
 // One step's projection rows [T, (nh + 2 nkv) * HD] (bf16, or S fp32 split-K planes that are summed
 // here): per-head RMS norm of q and k (optional), rotation, q out as bf16, k and v into the pages.
 // Everything between the load and the one rounding at the end is fp32.  HD / 8 lanes hold a head;
-// the rotation's partner dim (d, d + HD/2) is HD / 16 lanes away.
+// the rotation's partner dim (d, d + HD/2) is HD / 16 lanes away.  A block takes `steps` heads per lane
+// group of one token, so that the angles are loaded once for them: several for a prompt's rows, one for
+// a step's, where more blocks are worth more (8191 rows of 48 heads with their read-back: 85 us with one, 69 with
+// six).
 template <int HD, bool kPlanes>
 __global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
     bf16* __restrict__ q_out, const void* __restrict__ qkv, int S, const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, int64_t max_pos, const bf16* __restrict__ q_w, const bf16* __restrict__ k_w,
     float eps, uint8_t* __restrict__ kc, int16_t* __restrict__ kw, uint8_t* __restrict__ vc, int16_t* __restrict__ vw,
-    const int* __restrict__ slots, int T, int nh, int nkv, uint32_t bs, int64_t num_slots, int* status) {
+    const int* __restrict__ slots, int T, int nh, int nkv, int steps, uint32_t bs, int64_t num_slots, int* status) {
   pdl_trigger();
   pdl_wait();
-  constexpr int kLanes = HD / 8, kHalf = HD / 2;
-  const int heads = nh + 2 * nkv;
-  const uint32_t rows = (uint32_t)T * heads;
-  const uint32_t r0 = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  const bool live = r0 < rows;
-  const uint32_t r = live ? r0 : rows - 1;         // tail lanes take part in the butterflies
-  const int t = (int)(r / (uint32_t)heads), head = (int)(r - (uint32_t)t * heads);
+  constexpr int kLanes = HD / 8, kHalf = HD / 2, kGroups = kThreads / kLanes;
+  const int heads = nh + 2 * nkv, t = blockIdx.x;
+  const int head0 = blockIdx.y * kGroups * steps + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes, d0 = lane * 8;
-  float x[8];
-  if constexpr (kPlanes) {
-    const float* p = (const float*)qkv + (int64_t)r * HD + d0;
-    const int64_t plane = (int64_t)rows * HD;
+  auto load = [&](int head, float* x) {
+    const int64_t at = ((int64_t)t * heads + min(head, heads - 1)) * HD + d0;
+    if constexpr (kPlanes) {
+      const float* p = (const float*)qkv + at;
+      const int64_t plane = (int64_t)T * heads * HD;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < S; ++s) {
-      const float4 a = *reinterpret_cast<const float4*>(p + s * plane);
-      const float4 b = *reinterpret_cast<const float4*>(p + s * plane + 4);
-      x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w;
-      x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+      for (int s = 0; s < S; ++s) {
+        const float4 a = *reinterpret_cast<const float4*>(p + s * plane);
+        const float4 b = *reinterpret_cast<const float4*>(p + s * plane + 4);
+        x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w;
+        x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+      }
+    } else {
+      unpack_bf16x8(*reinterpret_cast<const uint4*>((const bf16*)qkv + at), x);
     }
-  } else {
-    unpack_bf16x8(*reinterpret_cast<const uint4*>((const bf16*)qkv + (int64_t)r * HD + d0), x);
-  }
-  const bool is_v = head >= nh + nkv;
-  const bf16* w = head < nh ? q_w : k_w;
-  if (w != nullptr) {                              // uniform over the grid: both or neither
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!is_v) {
-      const float inv = rsqrtf(ss / HD + eps);
-      float g[8];
-      unpack_bf16x8(*reinterpret_cast<const uint4*>(w + d0), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-    }
-  }
+  };
+  float x[8], c[8], s[8];
+  load(head0, x);
+  const int slot = slots[t];
   int64_t pos = positions[t];
   const bool pos_ok = pos >= 0 && pos < max_pos;
   if (!pos_ok) {                                   // never read outside the table; the row is not stored
-    if (live) record_error(status, kBadIndex);
+    if (head0 == 0) record_error(status, kBadIndex);
     pos = 0;
   }
-  float y[8];
+  const float* cs = cos_sin + pos * HD + (d0 & (kHalf - 1));
+  const float sign = d0 < kHalf ? -1.f : 1.f;      // x1 c - x2 s | x2 c + x1 s
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = __shfl_xor_sync(0xffffffffu, x[i], kLanes / 2);
-  if (!is_v) {
-    const float* cs = cos_sin + pos * HD + (d0 & (kHalf - 1));
-    const float sign = d0 < kHalf ? -1.f : 1.f;    // x1 c - x2 s | x2 c + x1 s
-    float c[8], s[8];
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + i);
+    const float4 v = *reinterpret_cast<const float4*>(cs + kHalf + i);
+    s[i] = sign * v.x, s[i + 1] = sign * v.y, s[i + 2] = sign * v.z, s[i + 3] = sign * v.w;
+  }
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    const int head = head0 + i * kGroups;
+    if (head - threadIdx.x / kLanes >= heads) break;       // the same for the whole block
+    float next[8];
+    if (i + 1 < steps) load(head + kGroups, next);
+    const bool live = head < heads, is_v = head >= nh + nkv;
+    if (q_w != nullptr) {                          // uniform over the grid: both weights or neither
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(cs + i);
-      *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(cs + kHalf + i);
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (!is_v) {
+        const float inv = rsqrtf(ss / HD + eps);
+        float g[8];
+        unpack_bf16x8(*reinterpret_cast<const uint4*>((head < nh ? q_w : k_w) + d0), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * g[e];
+      }
+    }
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __shfl_xor_sync(0xffffffffu, x[e], kLanes / 2);
+    if (!is_v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + y[e] * s[e];
+    uint32_t word = 0, codes = 0;
+    if (__any_sync(0xffffffffu, head >= nh)) {     // a warp of query heads has nothing to quantise
+      // values that are bf16 already (V of a bf16 projection) take the exact-tie form
+      const bool all_v = !kPlanes && __all_sync(0xffffffffu, is_v), some_v = !kPlanes && __any_sync(0xffffffffu, is_v);
+      if (!all_v) codes = quantise8<false>(x, word);
+      if (some_v) {
+        uint32_t word_v;
+        const uint32_t codes_v = quantise8<true>(x, word_v);
+        if (is_v) codes = codes_v, word = word_v;
+      }
+    }
+    if (live && head < nh) {
+      *reinterpret_cast<uint4*>(q_out + ((int64_t)t * nh + head) * HD + d0) =
+          pos_ok ? make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]))
+                 : make_uint4(0, 0, 0, 0);
+    } else if (live) {
+      const int h = is_v ? head - nh - nkv : head - nh;
+      size_t row;
+      if (pos_ok && page_row(slot, num_slots, nkv, h, bs, status, row)) {
+        reinterpret_cast<uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane] = codes;
+        if (lane % 8 == 0) (is_v ? vw : kw)[row * (HD / kGroup) + lane / 8] = (int16_t)word;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + sign * y[i] * s[i];
+    for (int e = 0; e < 8; ++e) x[e] = next[e];
   }
-  uint32_t word = 0, codes = 0;
-  if (__any_sync(0xffffffffu, head >= nh)) {       // a warp of query heads has nothing to quantise
-    // values that are bf16 already (V of a bf16 projection) take the exact-tie form
-    const bool all_v = !kPlanes && __all_sync(0xffffffffu, is_v), some_v = !kPlanes && __any_sync(0xffffffffu, is_v);
-    if (!all_v) codes = quantise8<false>(x, word);
-    if (some_v) {
-      uint32_t word_v;
-      const uint32_t codes_v = quantise8<true>(x, word_v);
-      if (is_v) codes = codes_v, word = word_v;
-    }
-  }
-  if (!live) return;
-  if (head < nh) {
-    *reinterpret_cast<uint4*>(q_out + ((int64_t)t * nh + head) * HD + d0) =
-        pos_ok ? make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]))
-               : make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const int h = is_v ? head - nh - nkv : head - nh;
-  size_t row;
-  if (!pos_ok || !page_row(slots[t], num_slots, nkv, h, bs, status, row)) return;
-  reinterpret_cast<uint32_t*>((is_v ? vc : kc) + row * (HD / 2))[lane] = codes;
-  if (lane % 8 == 0) (is_v ? vw : kw)[row * (HD / kGroup) + lane / 8] = (int16_t)word;
 }
 
 inline bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -377,16 +388,18 @@ void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::T
                                        aligned16(*w) && w->device() == dev),
                    "norm weights must be contiguous bfloat16 [head_dim]");
   if (T == 0) return;
-  const int64_t per = kThreads / (hd / 8), rows = T * (nh + 2 * nkv);
+  const int64_t rows = T * (nh + 2 * nkv), groups = kThreads / (hd / 8), chunks = (nh + 2 * nkv + groups - 1) / groups;
+  // heads per lane group: as many as leave sixteen blocks a SM
+  const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(chunks, T * chunks / (148 * 16)));
   LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
   const at::cuda::CUDAGuard g(dev);
   auto go = [&](auto kern) {
-    launch_pdl(kern, dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(),
+    launch_pdl(kern, dim3((unsigned)T, (unsigned)((chunks + steps - 1) / steps)), dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(),
                (bf16*)q_out.data_ptr(), (const void*)qkv.data_ptr(), (int)S, positions.data_ptr<int64_t>(),
                cos_sin.data_ptr<float>(), cos_sin.size(0), q_w.numel() ? (const bf16*)q_w.data_ptr() : nullptr,
                k_w.numel() ? (const bf16*)k_w.data_ptr() : nullptr, (float)eps, kc.data_ptr<uint8_t>(),
                kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), slots.data_ptr<int>(), (int)T,
-               (int)nh, (int)nkv, (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
+               (int)nh, (int)nkv, (int)steps, (uint32_t)kc.size(2), kc.size(0) * kc.size(2), status_ptr(status));
   };
   if (hd == 128) planes ? go(rope_store_int4_kernel<128, true>) : go(rope_store_int4_kernel<128, false>);
   else planes ? go(rope_store_int4_kernel<64, true>) : go(rope_store_int4_kernel<64, false>);
