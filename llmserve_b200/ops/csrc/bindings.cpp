@@ -90,8 +90,9 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
 void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                            int64_t nq, at::Tensor lens, at::Tensor tables, double scale, at::Tensor part_o,
                            at::Tensor part_ml, at::Tensor counters, int64_t max_splits, at::Tensor status);
-void step_maps(at::Tensor q_lens, at::Tensor k_lens, at::Tensor ids, int64_t bs, at::Tensor cu, at::Tensor positions,
-               at::Tensor slots, at::Tensor tables, at::Tensor last, at::Tensor status);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_maps(at::Tensor q_lens, at::Tensor k_lens,
+                                                                                 at::Tensor ids, int64_t bs, int64_t T,
+                                                                                 int64_t width, at::Tensor status);
 }  // namespace lsb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

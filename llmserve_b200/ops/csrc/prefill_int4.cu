@@ -136,7 +136,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     bf16* __restrict__ out, const bf16* __restrict__ q, Pages kp, Pages vp, const int* __restrict__ cu_q,
     const int* __restrict__ k_lens, const int* __restrict__ tables, int width, int B, int T, float scale_log2, int nh,
-    int nkv, int bs, int nblk, int pairs, int* __restrict__ status) {
+    int nkv, int bs, int nblk, int* __restrict__ status) {
   using L = PfLayout<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -153,12 +153,31 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
 
   pdl_trigger();
   pdl_wait();
-  // the blocks with most keys first: blockIdx.y enumerates (pair of tiles from the last, sequence)
-  const int pair = pairs - 1 - (int)blockIdx.y / B, seq = (int)blockIdx.y % B, kvh = blockIdx.x;
+  // This block's sequence and pair of tiles: the grid holds (pair of tiles, KV head), heads fastest, for as many
+  // pairs as the rows can make; a sequence's last pair, which sees most keys, comes first.
   const int G = nh / nkv, per_tile = kBQ / G;              // queries of a tile
+  const int kvh = blockIdx.x % nkv, want = blockIdx.x / nkv;
+  int seq = -1, pair = 0, base = 0;
+  for (int b0 = 0; b0 < B && seq < 0; b0 += 32) {
+    int n = 0;
+    if (b0 + lane < B) n = (max(0, min(cu_q[b0 + lane + 1], T) - max(0, min(T, cu_q[b0 + lane]))) + 2 * per_tile - 1) / (2 * per_tile);
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, base + incl > want);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = b0 + l;
+      pair = base + __shfl_sync(0xffffffffu, incl, l) - 1 - want;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (seq < 0) return;
   const int q0 = max(0, min(T, cu_q[seq])), q_len = min(cu_q[seq + 1], T) - q0;
   const int first = pair * 2 * per_tile;
-  if (first >= q_len) return;
   const int k_cap = max(0, min(k_lens[seq], (int)min((int64_t)width * bs, (int64_t)INT32_MAX - kBK)));
   const int shift = k_lens[seq] - q_len;                   // absolute position of query 0
   int kend_t[2], nt[2];
@@ -556,15 +575,17 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
   LSB_INT4_CHECK(kc.numel() / (hd / 2) / 16 < INT32_MAX && T < INT32_MAX, "pages exceed int32 rows of 16 keys");
   if (T == 0 || B == 0 || max_q <= 0) return;
   const at::cuda::CUDAGuard guard(dev);
-  const int64_t per = 2 * (kBQ / (nh / nkv)), pairs = (std::min(max_q, T) + per - 1) / per;
-  LSB_INT4_CHECK(pairs * B < 65536, "too many query tiles for one launch");
+  // pairs of tiles: every sequence ends one early, and none is longer than max_q
+  const int64_t per = 2 * (kBQ / (nh / nkv));
+  const int64_t pairs = std::min(T / per + B, (std::min(max_q, T) + per - 1) / per * B);
+  LSB_INT4_CHECK(pairs * nkv < INT32_MAX, "too many query tiles for one launch");
   auto go = [&](auto kern, int smem) {
     ensure_dynamic_smem((const void*)kern, smem);
-    launch_pdl(kern, dim3((unsigned)nkv, (unsigned)(pairs * B)), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(),
+    launch_pdl(kern, dim3((unsigned)(pairs * nkv)), dim3(kThreads), smem, at::cuda::getCurrentCUDAStream(),
                (bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), Pages{kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
                Pages{vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, (const int*)cu_q.data_ptr<int>(),
                (const int*)k_lens.data_ptr<int>(), (const int*)tables.data_ptr<int>(), (int)tables.size(1), (int)B, (int)T,
-               (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs, (int)kc.size(0), (int)pairs,
+               (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs, (int)kc.size(0),
                status_ptr(status));
   };
   if (hd == 128) go(prefill_int4_kernel<128>, PfLayout<128>::kBytes);

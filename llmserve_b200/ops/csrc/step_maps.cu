@@ -8,6 +8,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <tuple>
+
 #include "int4_pages.cuh"
 
 namespace lsb {
@@ -109,29 +111,27 @@ __global__ void __launch_bounds__(kThreads) step_maps_kernel(
 }  // namespace
 
 // q_lens / k_lens int32 [B] (new tokens, keys after the step); ids int32 [N]: each request's block ids
-// in order, ceil(k_len / block_size) of them, back to back.
-void step_maps(at::Tensor q_lens, at::Tensor k_lens, at::Tensor ids, int64_t bs, at::Tensor cu, at::Tensor positions,
-               at::Tensor slots, at::Tensor tables, at::Tensor last, at::Tensor status) {
+// in order, ceil(k_len / block_size) of them, back to back.  Returns cu_seqlens_q, positions, slot_mapping,
+// block_tables, last_token_indices (allocated here: five tensors from Python cost more than the kernel).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_maps(at::Tensor q_lens, at::Tensor k_lens,
+                                                                                 at::Tensor ids, int64_t bs, int64_t T,
+                                                                                 int64_t width, at::Tensor status) {
   const at::Device dev = q_lens.device();
   LSB_INT4_CHECK(q_lens.is_cuda(), "q_lens must be a CUDA tensor");
   int4::check_int32(q_lens, "q_lens", 1, dev);
   int4::check_int32(k_lens, "k_lens", 1, dev);
   int4::check_int32(ids, "block_ids", 1, dev);
-  int4::check_int32(cu, "cu_seqlens_q", 1, dev);
-  int4::check_int32(slots, "slot_mapping", 1, dev);
-  int4::check_int32(tables, "block_tables", 2, dev);
-  const int64_t B = q_lens.size(0), T = slots.size(0), width = tables.size(1);
-  for (const at::Tensor* t : {&positions, &last})
-    LSB_INT4_CHECK(t->scalar_type() == at::kLong && t->is_contiguous() && t->dim() == 1 && t->device() == dev,
-                   "positions and last_token_indices must be contiguous int64");
-  LSB_INT4_CHECK(k_lens.size(0) == B && cu.size(0) == B + 1 && tables.size(0) == B && last.size(0) == B &&
-                     positions.size(0) == T,
-                 "step map sizes do not match");
+  const int64_t B = q_lens.size(0);
+  LSB_INT4_CHECK(k_lens.size(0) == B, "q_lens and k_lens differ in length");
   LSB_INT4_CHECK(bs >= 1 && bs <= INT32_MAX, "block_size must be positive");
+  LSB_INT4_CHECK(T >= 0 && width >= 0, "num_tokens and table_width must not be negative");
   LSB_INT4_CHECK(B <= kMaxRequests, "more than 8192 requests in one step");
   LSB_INT4_CHECK(T <= INT32_MAX - (1 << 20) && B * width <= INT32_MAX - (1 << 20) && ids.size(0) <= INT32_MAX,
                  "step maps exceed int32");
   const at::cuda::CUDAGuard g(dev);
+  const auto i32 = q_lens.options(), i64 = i32.dtype(at::kLong);
+  at::Tensor cu = at::empty({B + 1}, i32), positions = at::empty({T}, i64), slots = at::empty({T}, i32),
+             tables = at::empty({B, width}, i32), last = at::empty({B}, i64);
   const int64_t items = std::max(std::max(T, B * width), B + 1);
   // four items to a thread: a block's scan of the lengths is worth a thousand of them
   const unsigned grid = (unsigned)std::min<int64_t>(148, (items + 4 * kThreads - 1) / (4 * kThreads));
@@ -143,6 +143,7 @@ void step_maps(at::Tensor q_lens, at::Tensor k_lens, at::Tensor ids, int64_t bs,
              tables.data_ptr<int>(), last.data_ptr<int64_t>(), status_ptr(status));
   const cudaError_t e = cudaGetLastError();
   LSB_INT4_CHECK(e == cudaSuccess, std::string("step_maps launch failed: ") + cudaGetErrorString(e));
+  return {cu, positions, slots, tables, last};
 }
 
 }  // namespace lsb

@@ -73,6 +73,14 @@ def _check_pages(k_pages, v_pages, nkv=None, hd=None):
         raise ValueError("head layout does not match the pages")
 
 
+def _check_query(q, k_pages, v_pages, scale):
+    _check_pages(k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != k_pages.shape[3] or q.shape[1] < 1 or q.shape[1] % k_pages.shape[1]:
+        raise ValueError("query heads do not match the pages")
+    if not 0 < scale < float("inf"):
+        raise ValueError("scale must be positive")
+
+
 # ---- fp32 restatement (the CPU path) -----------------------------------------------------------
 def quantise_int4_ref(x: torch.Tensor):
     """Rows ``[..., head_dim]`` -> (codes, words) of the page format, computed in fp32."""
@@ -207,7 +215,7 @@ def verify_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table
     if nq < 1 or q.shape[0] != seqlens_k.shape[0] * nq:
         raise ValueError("q must hold nq >= 1 rows per sequence")
     if not q.is_cuda:
-        _check_pages(k_pages, v_pages, None, None)
+        _check_query(q, k_pages, v_pages, scale)
         cu = torch.arange(0, q.shape[0] + 1, nq, dtype=torch.int32)
         return attention_int4_ref(q, k_pages, v_pages, cu, seqlens_k, block_tables, scale)
     rows, nh, hd = q.shape
@@ -249,7 +257,7 @@ def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens
     sees keys ``< seqlens_k - q_len + j + 1``.  ``max_seqlen_q`` is at least the longest chunk (rows past
     it, like rows behind the last sequence, are left unwritten)."""
     if not q.is_cuda:
-        _check_pages(k_pages, v_pages)
+        _check_query(q, k_pages, v_pages, scale)
         return attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_tables, scale)
     out = torch.empty_like(q)
     C().prefill_attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words,

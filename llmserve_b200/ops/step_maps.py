@@ -66,13 +66,4 @@ def build_step_maps(q_lens: torch.Tensor, k_lens: torch.Tensor, block_ids: torch
     if not q_lens.is_cuda:
         _check(q_lens, k_lens, block_ids, block_size, num_tokens, table_width)
         return build_step_maps_ref(q_lens, k_lens, block_ids, block_size, num_tokens, table_width)
-    d, n = q_lens.device, q_lens.shape[0]
-    if num_tokens < 0 or table_width < 0:
-        raise ValueError("num_tokens and table_width must not be negative")
-    m = StepMaps(torch.empty(n + 1, dtype=torch.int32, device=d),
-                 torch.empty(num_tokens, dtype=torch.int64, device=d),
-                 torch.empty(num_tokens, dtype=torch.int32, device=d),
-                 torch.empty(n, table_width, dtype=torch.int32, device=d),
-                 torch.empty(n, dtype=torch.int64, device=d))
-    C().step_maps(q_lens, k_lens, block_ids, block_size, *m, status(d))
-    return m
+    return StepMaps(*C().step_maps(q_lens, k_lens, block_ids, block_size, num_tokens, table_width, status(q_lens.device)))

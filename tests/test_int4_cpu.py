@@ -104,6 +104,9 @@ def test_refusals():
         kv_int4.store_kvcache_int4(k, k, kp.codes, vp, s)
     with pytest.raises(ValueError, match="nq"):
         kv_int4.verify_attention_int4(_rows(5, 2, 64), kp, vp, s[None], s[:2], 1.0, 2)
+    for q, scale in ((_rows(2, 3, 64), 1.0), (_rows(2, 2, 128), 1.0), (_rows(2, 2, 64), 0.0)):
+        with pytest.raises(ValueError):
+            kv_int4.decode_attention_int4(q, kp, vp, s[:, None], s, scale)
     i = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
     for q, n, ids, rows in ((i(3), i(2), i(0), 3), (i(-1), i(2), i(0), 3), (i(2), i(2), i(0), 1), (i(2), i(17), i(0), 2)):
         with pytest.raises(ValueError):

@@ -263,6 +263,39 @@ def test_prefill_long_chunk_and_rows_without_keys():
     assert out[700:705].eq(0).all()
 
 
+@pytest.mark.parametrize("kind", ["prefill", "verify"])
+def test_a_nan_token_reaches_only_the_rows_that_see_it(kind):
+    """Token 40 of 64 holds NaN in the second group of its V: rows before it are untouched, rows from it on
+    are NaN in that group's dims of that KV head's queries and right elsewhere."""
+    n, new = 64, 64 if kind == "prefill" else 30
+    q, kp, vp, cu, tables = _case(1, 4, 2, 128, 16, [new], [n], 21)
+    at = tables[0, 40 // 16], 1, 40 % 16
+    whole = vp[1][at].clone()
+    vp[1][at][1] = 0x7FC0
+    args = (q.to(DEV), _on(kp), _on(vp))
+    if kind == "prefill":
+        out = kv_int4.prefill_attention_int4(*args, _i32(*cu), _i32(n), tables.to(DEV), 0.09, new)
+    else:
+        out = kv_int4.verify_attention_int4(*args, tables.to(DEV), _i32(n), 0.09, new)
+    vp[1][at] = whole
+    want, mag = oracle.attention(q, kp, vp, cu, [n], tables, 0.09)
+    nan = torch.zeros_like(out, dtype=torch.bool)
+    nan[40 - (n - new):, 2:, 64:] = True
+    assert torch.equal(out.isnan(), nan)
+    keep = ~nan.cpu()
+    assert ((out.double().cpu() - want).abs() <= oracle.attention_tolerance(want, mag))[keep].all()
+
+
+def test_prefill_of_many_ragged_sequences():
+    q_lens = [(i * 7) % 5 for i in range(300)]
+    q_lens[150] = 400
+    k_lens = [n + (i * 13) % 40 for i, n in enumerate(q_lens)]
+    q, kp, vp, cu, tables = _case(300, 8, 1, 64, 16, q_lens, k_lens, 2)
+    want, mag = oracle.attention(q, kp, vp, cu, k_lens, tables, 0.125)
+    out = kv_int4.prefill_attention_int4(q.to(DEV), _on(kp), _on(vp), _i32(*cu), _i32(*k_lens), tables.to(DEV), 0.125, 400)
+    _assert_close(out, want, mag)
+
+
 def test_strong_scores_and_extreme_scales():
     """Scores in the hundreds (one key takes all), V scales from 1e-30 to 1e30."""
     q, kp, vp, cu, tables = _case(3, 8, 2, 128, 16, [1, 1, 1], [40, 300, 77], 9)
