@@ -79,8 +79,8 @@ void kv_push(at::Tensor src_k, at::Tensor src_v, at::Tensor dst_k, at::Tensor ds
              at::Tensor dst_ids, at::Tensor status);
 void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                         at::Tensor slots, at::Tensor status);
-void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
-                       at::Tensor slots, at::Tensor status);
+std::tuple<at::Tensor, at::Tensor> load_kvcache_int4(at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                                                     at::Tensor slots, at::Tensor status);
 void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,
                    at::Tensor k_w, double eps, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                    at::Tensor slots, int64_t nh, at::Tensor status);

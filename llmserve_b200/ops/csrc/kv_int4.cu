@@ -7,6 +7,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <tuple>
+
 #include "int4_pages.cuh"
 
 namespace lsb {
@@ -334,18 +336,17 @@ void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw
   launch_check("store_kvcache_int4");
 }
 
-void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
-                       at::Tensor slots, at::Tensor status) {
-  check_page_pair(kc, kw, vc, vw, k.device());
-  check_int32(slots, "slot_mapping", 1, k.device());
-  LSB_INT4_CHECK(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 3 &&
-                     k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.device() == k.device() &&
-                     k.size(0) == slots.size(0) && k.size(1) == kc.size(1) && k.size(2) == kc.size(3) * 2,
-                 "outputs must be contiguous bfloat16 [slots, kv_heads, head_dim]");
+std::tuple<at::Tensor, at::Tensor> load_kvcache_int4(at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                                                     at::Tensor slots, at::Tensor status) {
+  const at::Device dev = kc.device();
+  check_page_pair(kc, kw, vc, vw, dev);
+  check_int32(slots, "slot_mapping", 1, dev);
+  const at::cuda::CUDAGuard g(dev);
+  at::Tensor k = at::empty({slots.size(0), kc.size(1), kc.size(3) * 2}, kc.options().dtype(at::kBFloat16)),
+             v = at::empty_like(k);
   const int64_t rows = k.size(0) * k.size(1), per = kThreads / (k.size(2) / 8);
-  if (rows == 0) return;
+  if (rows == 0) return {k, v};
   LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
-  const at::cuda::CUDAGuard g(k.device());
   const dim3 grid((unsigned)((rows + per - 1) / per));
   auto go = [&](auto kern) {
     launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (bf16*)k.data_ptr(),
@@ -356,6 +357,7 @@ void load_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw,
   if (k.size(2) == 128) go(load_int4_kernel<128>);
   else go(load_int4_kernel<64>);
   launch_check("load_kvcache_int4");
+  return {k, v};
 }
 
 void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,

@@ -165,11 +165,7 @@ def load_kvcache_int4(k_pages: Int4Pages, v_pages: Int4Pages, slot_mapping):
     if not codes.is_cuda:
         _check_pages(k_pages, v_pages)
         return load_kv_int4_ref(k_pages, v_pages, slot_mapping)
-    k = torch.empty(slot_mapping.shape[0], codes.shape[1], 2 * codes.shape[3], dtype=torch.bfloat16,
-                    device=codes.device)
-    v = torch.empty_like(k)
-    C().load_kvcache_int4(k, v, codes, k_pages.words, v_pages.codes, v_pages.words, slot_mapping, status(codes.device))
-    return k, v
+    return C().load_kvcache_int4(codes, k_pages.words, v_pages.codes, v_pages.words, slot_mapping, status(codes.device))
 
 
 _NO_WEIGHT = {}

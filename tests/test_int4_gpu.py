@@ -335,6 +335,50 @@ def test_block_ids_outside_the_pool_are_not_seen_and_long_contexts_end_at_their_
     _assert_close(out, want, mag)
 
 
+def test_offsets_past_32_bits():
+    """Pools of 2.4 GB of codes each: the last blocks lie more than 2^31 bytes from the first."""
+    nkv, bs, hd, blocks = 8, 16, 128, 290000
+    n = 75
+    q, kp, vp, cu, tables = _case(1, 16, nkv, hd, bs, [9], [n], 31, spare=0)
+    small = kp[0].shape[0]
+    big = [_pages((blocks, nkv, bs, hd)) for _ in range(2)]
+    for p, b in zip((kp, vp), big):
+        b.codes[blocks - small:], b.words[blocks - small:] = p[0].to(DEV), p[1].to(DEV)
+    far = (tables + blocks - small).to(DEV)
+    want, mag = oracle.attention(q, kp, vp, cu, [n], tables, 0.09)
+    _assert_close(kv_int4.prefill_attention_int4(q.to(DEV), *big, _i32(*cu), _i32(n), far, 0.09, 9), want, mag)
+    _assert_close(kv_int4.verify_attention_int4(q.to(DEV), *big, far, _i32(n), 0.09, 9), want, mag)
+    x = torch.randn(2, nkv, hd, device=DEV).bfloat16()
+    slots = _i32(blocks * bs - 1, 3)
+    kv_int4.store_kvcache_int4(x, -x, *big, slots)
+    k, v = kv_int4.load_kvcache_int4(*big, slots)
+    assert torch.equal(k.double().cpu(), _dequantised(x)) and torch.equal(v.double().cpu(), _dequantised(-x))
+    qkv = torch.randn(2, 18 * hd, device=DEV).bfloat16()
+    kv_int4.qkv_norm_rope_store_int4(qkv, torch.zeros(2, dtype=torch.long, device=DEV),
+                                     rope.build_cos_sin_cache(hd, 4, 1e4).to(DEV), None, None, 1e-6, *big, slots, 2, nkv, hd)
+    v = kv_int4.load_kvcache_int4(*big, slots)[1]
+    assert torch.equal(v.double().cpu(), _dequantised(qkv[:, 10 * hd:].reshape(2, nkv, hd)))
+
+
+def test_two_streams_with_a_workspace_each():
+    lens = [900, 33, 4000]
+    q, kp, vp, cu, tables = _case(3, 8, 2, 128, 64, [1] * 3, lens, 12)
+    want, mag = oracle.attention(q, kp, vp, cu, lens, tables, 0.09)
+    qd, k, v, t, n = q.to(DEV), _on(kp), _on(vp), tables.to(DEV), _i32(*lens)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    spaces = [DecodeWorkspace(3, 8, 128, tables.shape[1] * 64, DEV) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for stream, w in zip(streams, spaces):
+            with torch.cuda.stream(stream):
+                outs.append(kv_int4.decode_attention_int4(qd, k, v, t, n, 0.09, w))
+    torch.cuda.synchronize()
+    _assert_close(outs[0], want, mag)
+    # pieces are merged in their order: the same bits every time
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 def test_captured_decode_replays_on_new_lengths_and_side_streams():
     lens = [300, 0, 17, 512]
     q, kp, vp, cu, tables = _case(4, 8, 2, 128, 64, [1] * 4, [512] * 4, 8)
