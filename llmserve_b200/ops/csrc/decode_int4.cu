@@ -23,11 +23,13 @@
 // shares over a grid that fills the GPU once, whatever the lengths: lengths are read on the device, so one
 // captured launch serves any batch.  A (sequence, head) that is cut leaves fp32 partials; the block that
 // finishes last merges them in their order (results do not depend on who is last) and resets the counter.
-// Where every (sequence, head) can have a block and none is more than kCutCost chunks above the equal share,
-// nothing is cut: leaving and merging a piece costs about as much as that many chunks.
+// Where every (sequence, head) can have a block and none is far above the equal share, nothing is cut: leaving
+// and merging a piece costs about kCutCost chunks, and kNextCost more where a block goes on to another one
+// (on the device, cut / not: one context of 513 keys 10.4 / 11.4 us, eight of 700 15.7 / 17.1, 64 of 600 to 1200
+// 33.8 / 29.8, 64 of 256 to 512 cut by an earlier form 25.6 / 17.6).
 //
 // Measured on a B200 with 32 query and 8 KV heads of 128: 32 contexts of 1..32768 keys 171 us (594 MB: 3.5 TB/s),
-// 64 of 256..512 keys 18 us (25.6 with every pair cut), 64 x 4 queries on 200..2048 keys 79 us.
+// 64 of 256..512 keys 18 us, 64 x 4 queries on 200..2048 keys 79 us.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -53,7 +55,7 @@ constexpr int kWarpKeys = kChunk / kWarps;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlocksPerSm = 4;           // 128 registers a thread
 constexpr int kRows = 8;                  // query rows of a block
-constexpr int kCutCost = 3;
+constexpr int kCutCost = 3, kNextCost = 2;
 constexpr float kRescaleLog2 = 8.f;
 
 template <int HD>
@@ -160,7 +162,7 @@ __device__ __forceinline__ Share find_share(const Args& a, int lane, Deal& deal)
   most = __reduce_max_sync(0xffffffffu, most);
   Share s = {0, 0, 0, 0};
   const int blocks = (int)gridDim.x, me = (int)blockIdx.x;
-  const bool uncut = (int64_t)a.B * a.nkv <= blocks && most <= deal.total / blocks + kCutCost;
+  const bool uncut = (int64_t)a.B * a.nkv <= blocks && most <= deal.total / blocks + kCutCost + (deal.total > blocks ? kNextCost : 0);
   deal.grid = uncut ? 0 : min(blocks, deal.total);
   if (uncut ? me >= a.B * a.nkv : me >= deal.grid) return s;
   if (!uncut) {
