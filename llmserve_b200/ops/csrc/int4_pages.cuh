@@ -17,9 +17,6 @@ namespace int4 {
 
 constexpr int kGroup = 64;
 
-__device__ __forceinline__ float word_scale(uint32_t w) { return __uint_as_float((w & 0x7ff0u) << 16); }
-__device__ __forceinline__ uint32_t word_zero(uint32_t w) { return w & 15u; }
-
 struct Pages {
   const uint8_t* codes;
   const int16_t* words;
