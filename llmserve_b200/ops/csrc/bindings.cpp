@@ -90,6 +90,8 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
 void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                            int64_t nq, at::Tensor lens, at::Tensor tables, double scale, at::Tensor part_o,
                            at::Tensor part_ml, at::Tensor counters, int64_t max_splits, at::Tensor status);
+void commit_tree_kv_int4(at::Tensor tkc, at::Tensor tkw, at::Tensor tvc, at::Tensor tvw, at::Tensor kc, at::Tensor kw,
+                         at::Tensor vc, at::Tensor vw, at::Tensor nodes, at::Tensor slots, at::Tensor status);
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_maps(at::Tensor q_lens, at::Tensor k_lens,
                                                                                  at::Tensor ids, int64_t bs, int64_t T,
                                                                                  int64_t width, at::Tensor status);
@@ -146,6 +148,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_rope_int4", &lsb::qkv_rope_int4);
   m.def("prefill_attention_int4", &lsb::prefill_attention_int4);
   m.def("decode_attention_int4", &lsb::decode_attention_int4);
+  m.def("commit_tree_kv_int4", &lsb::commit_tree_kv_int4);
   m.def("step_maps", &lsb::step_maps);
   m.def("greedy_accept", &lsb::greedy_accept);
   m.def("gemm_bf16", &lsb::gemm_bf16, py::arg("out"), py::arg("x"), py::arg("w"), py::arg("partials"),

@@ -292,6 +292,33 @@ __global__ void __launch_bounds__(kThreads) rope_store_int4_kernel(
   }
 }
 
+// Accepted tree nodes' rows of every layer into the pools, codes and words as they are (quantising what was
+// quantised before need not give the same codes).  grid (layers, committed nodes, kv heads); lanes 0..15 take K,
+// 16..31 V.  A few kilobytes: launch latency bounds it.
+__global__ void commit_tree_int4_kernel(
+    const uint8_t* __restrict__ tkc, const int16_t* __restrict__ tkw, const uint8_t* __restrict__ tvc,
+    const int16_t* __restrict__ tvw, uint8_t* __restrict__ kc, int16_t* __restrict__ kw, uint8_t* __restrict__ vc,
+    int16_t* __restrict__ vw, const int* __restrict__ nodes, const int* __restrict__ slots, int n_nodes, int nkv, int hd,
+    uint32_t bs, int64_t num_slots, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  const int layer = blockIdx.x, h = blockIdx.z, lane = threadIdx.x & 15;
+  const bool is_v = threadIdx.x >= 16;
+  const int node = nodes[blockIdx.y];
+  if (node < 0 || node >= n_nodes) {
+    if (threadIdx.x == 0) record_error(status, kBadIndex);
+    return;
+  }
+  size_t to;
+  if (!page_row(slots[blockIdx.y], num_slots, nkv, h, bs, status, to)) return;
+  to += (size_t)layer * num_slots * nkv;
+  const size_t from = ((size_t)layer * n_nodes + node) * nkv + h;
+  if (lane < hd / 8)
+    reinterpret_cast<uint32_t*>((is_v ? vc : kc) + to * (hd / 2))[lane] =
+        reinterpret_cast<const uint32_t*>((is_v ? tvc : tkc) + from * (hd / 2))[lane];
+  if (lane < hd / kGroup) (is_v ? vw : kw)[to * (hd / kGroup) + lane] = (is_v ? tvw : tkw)[from * (hd / kGroup) + lane];
+}
+
 inline bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // [T, nkv, hd] rows whose last dim is dense and whose rows start on 16 bytes, else a dense copy
@@ -406,6 +433,40 @@ void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::T
   if (hd == 128) planes ? go(rope_store_int4_kernel<128, true>) : go(rope_store_int4_kernel<128, false>);
   else planes ? go(rope_store_int4_kernel<64, true>) : go(rope_store_int4_kernel<64, false>);
   launch_check("qkv_rope_int4");
+}
+
+// tree rows [layers, nodes, kv_heads, ..] into pools [layers, blocks, kv_heads, block_size, ..]
+void commit_tree_kv_int4(at::Tensor tkc, at::Tensor tkw, at::Tensor tvc, at::Tensor tvw, at::Tensor kc, at::Tensor kw,
+                         at::Tensor vc, at::Tensor vw, at::Tensor nodes, at::Tensor slots, at::Tensor status) {
+  const at::Device dev = kc.device();
+  LSB_INT4_CHECK(kc.dim() == 5 && kw.dim() == 5 && vc.dim() == 5 && vw.dim() == 5 && kc.is_contiguous() && kw.is_contiguous() &&
+                     vc.is_contiguous() && vw.is_contiguous(),
+                 "pools must be contiguous [layers, blocks, kv_heads, block_size, ..]");
+  const int64_t L = kc.size(0), nkv = kc.size(2), hd = kc.size(4) * 2, m = nodes.numel();
+  if (L == 0) return;
+  check_page_pair(kc[0], kw[0], vc[0], vw[0], dev);
+  LSB_INT4_CHECK(kw.size(0) == L && vc.size(0) == L && vw.size(0) == L, "pools differ in layers");
+  LSB_INT4_CHECK(tkc.dim() == 4 && tkc.size(0) == L && tkc.size(2) == nkv && tkc.size(3) * 2 == hd && tvc.sizes() == tkc.sizes() &&
+                     tkw.sizes() == at::IntArrayRef({L, tkc.size(1), nkv, hd / kGroup}) && tvw.sizes() == tkw.sizes(),
+                 "tree rows must be [layers, nodes, kv_heads, ..] of the pools' heads");
+  for (const at::Tensor* t : {&tkc, &tvc})
+    LSB_INT4_CHECK(t->scalar_type() == at::kByte && t->is_contiguous() && t->device() == dev && aligned16(*t),
+                   "tree codes must be contiguous, 16-byte aligned uint8 on the pools' device");
+  for (const at::Tensor* t : {&tkw, &tvw})
+    LSB_INT4_CHECK(t->scalar_type() == at::kShort && t->is_contiguous() && t->device() == dev,
+                   "tree scale words must be contiguous int16 on the pools' device");
+  check_int32(nodes, "node_indices", 1, dev);
+  check_int32(slots, "slot_mapping", 1, dev);
+  LSB_INT4_CHECK(slots.numel() == m, "slot_mapping must hold one slot per node");
+  LSB_INT4_CHECK(m <= 65535 && nkv <= 65535 && L <= INT32_MAX && tkc.size(1) <= INT32_MAX, "too many nodes or heads for one launch");
+  if (m == 0 || nkv == 0) return;
+  const at::cuda::CUDAGuard g(dev);
+  launch_pdl(commit_tree_int4_kernel, dim3((unsigned)L, (unsigned)m, (unsigned)nkv), dim3(32), 0,
+             at::cuda::getCurrentCUDAStream(), tkc.data_ptr<uint8_t>(), tkw.data_ptr<int16_t>(), tvc.data_ptr<uint8_t>(),
+             tvw.data_ptr<int16_t>(), kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>(), vc.data_ptr<uint8_t>(),
+             vw.data_ptr<int16_t>(), nodes.data_ptr<int>(), slots.data_ptr<int>(), (int)tkc.size(1), (int)nkv, (int)hd,
+             (uint32_t)kc.size(3), kc.size(1) * kc.size(3), status_ptr(status));
+  launch_check("commit_tree_kv_int4");
 }
 
 }  // namespace lsb

@@ -12,6 +12,7 @@ bfloat16 pattern of the group's scale ``s`` with the four low mantissa bits repl
 * ``qkv_norm_rope_store_int4``  -- one step's projection: QK-norm, RoPE, query out, K/V into the pages.
 * ``decode_attention_int4``     -- one query per sequence; ``verify_attention_int4``: ``nq`` of them.
 * ``tree_attention_int4``       -- EAGLE3 tree verify on a 4-bit prefix.
+* ``commit_tree_kv_int4``       -- copy accepted tree nodes, quantised when they were verified, into the pools.
 * ``prefill_attention_int4``    -- ragged causal chunks, on a cached prefix or without.
 
 On CUDA a slot or block id outside the pool is skipped (its keys are not seen) and recorded for
@@ -56,6 +57,10 @@ class Int4Pages:
 
     def __getitem__(self, layer) -> "Int4Pages":
         return Int4Pages(self.codes[layer], self.words[layer])
+
+    def rows(self, n: int) -> "Int4Pages":
+        """The first ``n`` rows of a pool of one block, as logical rows ``[n, kv_heads, head_dim]``."""
+        return Int4Pages(self.codes[0, :, :n].transpose(0, 1), self.words[0, :, :n].transpose(0, 1))
 
 
 def _check_pages(k_pages, v_pages, nkv=None, hd=None):
@@ -125,6 +130,16 @@ def load_kv_int4_ref(k_pages, v_pages, slot_mapping, dtype=torch.bfloat16):
         x[slots < 0] = 0
         out.append(x.to(dtype))
     return tuple(out)
+
+
+def commit_tree_kv_int4_ref(tree_k, tree_v, k_pages, v_pages, node_indices, slot_mapping):
+    bs = k_pages.shape[3]
+    for node, slot in zip(node_indices.tolist(), slot_mapping.tolist()):
+        if slot < 0:
+            continue
+        for x, p in ((tree_k, k_pages), (tree_v, v_pages)):
+            p.codes[:, slot // bs, :, slot % bs] = x.codes[:, node]
+            p.words[:, slot // bs, :, slot % bs] = x.words[:, node]
 
 
 def attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_tables, scale):
@@ -234,7 +249,9 @@ def decode_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table
 def tree_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table, prefix_len, tree_k, tree_v, tree_mask,
                         scale, mask_bits=None):
     """Tree verify on a 4-bit prefix: the sequence's pages are read back once (exact in bfloat16) and
-    ``ops.attention.tree_attention`` runs on the copy."""
+    ``ops.attention.tree_attention`` runs on the copy.  ``tree_k`` / ``tree_v`` are attended as they are
+    given: a node stands for the token that decode would write and read back, so its rows have to be
+    what pages hold of them (``qkv_norm_rope_store_int4`` into scratch pages, then ``load_kvcache_int4``)."""
     bs = k_pages.shape[2]
     n = max(1, -(-prefix_len // bs))
     if not q.is_cuda:
@@ -245,6 +262,30 @@ def tree_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table, 
         k, v = (x.unflatten(0, (-1, bs)).transpose(1, 2).contiguous() for x in load_kvcache_int4(k_pages, v_pages, slots))
     table = torch.arange(n, dtype=torch.int32, device=q.device)
     return attn_ops.tree_attention(q, k, v, table, prefix_len, tree_k, tree_v, tree_mask, scale, mask_bits)
+
+
+def commit_tree_kv_int4(tree_k: Int4Pages, tree_v: Int4Pages, k_pages: Int4Pages, v_pages: Int4Pages, node_indices,
+                        slot_mapping):
+    """Copy rows ``node_indices`` int32 [m] of every layer's tree nodes (``[layers, nodes, kv_heads, head_dim]``)
+    into the pools ``[layers, blocks, kv_heads, block_size, head_dim]`` at ``slot_mapping`` int32 [m]: codes
+    and words as they are, so that an accepted node reads back as it was attended."""
+    for x in (tree_k, tree_v, k_pages, v_pages):
+        if not isinstance(x, Int4Pages):
+            raise ValueError("tree K/V and pools must be Int4Pages")
+    t, p = tree_k.shape, k_pages.shape
+    if len(t) != 4 or tree_v.shape != t:
+        raise ValueError("tree K/V must be [layers, nodes, kv_heads, head_dim]")
+    if len(p) != 5 or v_pages.shape != p:
+        raise ValueError("target K/V pages must be [layers, blocks, kv_heads, block_size, head_dim]")
+    if (t[0], t[2], t[3]) != (p[0], p[2], p[4]):
+        raise ValueError("tree K/V and target pages differ in layers or heads")
+    if node_indices.ndim != 1 or node_indices.shape != slot_mapping.shape:
+        raise ValueError("selected nodes and slots must have matching one-dimensional shapes")
+    if not k_pages.codes.is_cuda:
+        return commit_tree_kv_int4_ref(tree_k, tree_v, k_pages, v_pages, node_indices, slot_mapping)
+    C().commit_tree_kv_int4(tree_k.codes.contiguous(), tree_k.words.contiguous(), tree_v.codes.contiguous(),
+                            tree_v.words.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words,
+                            node_indices, slot_mapping, status(k_pages.codes.device))
 
 
 def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens_q, seqlens_k, block_tables, scale,

@@ -6,7 +6,8 @@ during a tree verify every target attention layer keeps the K/V of all tree node
 acceptance :meth:`TreeKVCacheManager.commit` checks the captures, copies the selected nodes of
 every layer into their slots with one kernel (``ops.kv.commit_tree_kv``: grid over layers x
 nodes, 16-byte vector copies) and clears the captures whether or not the commit succeeded, so a
-failed step never leaves stale tree K/V behind.
+failed step never leaves stale tree K/V behind.  Captures for 4-bit pools are rows of 4-bit pages,
+whose codes and words are copied as they are (``ops.kv_int4.commit_tree_kv_int4``).
 """
 from collections.abc import Sequence
 
@@ -31,8 +32,7 @@ class TreeKVCacheManager:
 
     def clear(self):
         for layer in self.attention_layers:
-            layer.tree_k = layer.tree_k.new_empty(0)
-            layer.tree_v = layer.tree_v.new_empty(0)
+            layer.tree_k, layer.tree_v = (getattr(x, "codes", x).new_empty(0) for x in (layer.tree_k, layer.tree_v))
 
     def _check(self, node_indices: list[int], slot_mapping: torch.Tensor) -> int:
         if slot_mapping.ndim != 1 or slot_mapping.numel() != len(node_indices):
@@ -58,9 +58,15 @@ class TreeKVCacheManager:
             if self.k_cache is None or self.v_cache is None:
                 raise ValueError("a tree K/V commit needs the target K/V pools")
             if isinstance(self.k_cache, kv_int4.Int4Pages):
-                for i, layer in enumerate(self.attention_layers):
-                    kv_int4.store_kvcache_int4(layer.tree_k[node_indices], layer.tree_v[node_indices], self.k_cache[i],
-                                               self.v_cache[i], slot_mapping)
+                if not all(isinstance(layer.tree_k, kv_int4.Int4Pages) and isinstance(layer.tree_v, kv_int4.Int4Pages)
+                           for layer in self.attention_layers):
+                    raise ValueError("4-bit pools take tree captures in 4-bit pages")
+                tree_k, tree_v = (
+                    kv_int4.Int4Pages(torch.stack([x.codes for x in rows]), torch.stack([x.words for x in rows]))
+                    for rows in ([layer.tree_k for layer in self.attention_layers],
+                                 [layer.tree_v for layer in self.attention_layers]))
+                nodes = torch.tensor(node_indices, dtype=torch.int32, device=tree_k.codes.device)
+                kv_int4.commit_tree_kv_int4(tree_k, tree_v, self.k_cache, self.v_cache, nodes, slot_mapping)
                 return
             tree_k = torch.stack([layer.tree_k for layer in self.attention_layers])
             tree_v = torch.stack([layer.tree_v for layer in self.attention_layers])

@@ -1,0 +1,105 @@
+"""Tree verify on 4-bit pages on the GPU: nodes as decode stores them, and their commit."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from llmserve_b200.layers.attention import Attention  # noqa: E402
+from llmserve_b200.ops import kv_int4, rope  # noqa: E402
+from llmserve_b200.ops._ext import C, check_status  # noqa: E402
+from llmserve_b200.ops.kv_int4 import Int4Pages  # noqa: E402
+from llmserve_b200.speculative.tree import build_fixed_tree_topology  # noqa: E402
+from llmserve_b200.speculative.tree_kv import TreeKVCacheManager  # noqa: E402
+from llmserve_b200.utils.context import reset_context, set_context  # noqa: E402
+from tests import int4_oracle as oracle  # noqa: E402
+
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    C()
+    yield
+    check_status(torch.device(DEV))
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _on(p):
+    return Int4Pages(p[0].to(DEV), p[1].to(DEV))
+
+
+@pytest.mark.parametrize("nkv,hd,bs", [(3, 64, 16), (8, 128, 48), (1, 128, 256)])
+def test_commit_copies_the_chosen_rows_of_every_layer(nkv, hd, bs):
+    L, blocks, n = 3, 2, 11
+    tk, tv = (_on(oracle.random_pages(L, n, nkv, hd, s)) for s in (1, 2))
+    # rows of a step's scratch pages are strided
+    tk = Int4Pages(tk.codes.transpose(1, 2).contiguous().transpose(1, 2), tk.words.transpose(1, 2).contiguous().transpose(1, 2))
+    cpu = [oracle.random_pages(L * blocks, nkv, bs, hd, s) for s in (3, 4)]
+    k, v = (Int4Pages(*(x.to(DEV).view(L, blocks, nkv, bs, -1) for x in p)) for p in cpu)
+    want = [Int4Pages(*(x.clone().view(L, blocks, nkv, bs, -1) for x in p)) for p in cpu]
+    nodes, slots = _i32(10, 0, 4, 5), _i32(bs + 1, 2, -1, 2 * bs - 1)
+    kv_int4.commit_tree_kv_int4(tk, tv, k, v, nodes, slots)
+    kv_int4.commit_tree_kv_int4_ref(*(Int4Pages(x.codes.cpu(), x.words.cpu()) for x in (tk, tv)), *want, nodes.cpu(), slots.cpu())
+    for a, b in zip((k, v), want):
+        assert torch.equal(a.codes.cpu(), b.codes) and torch.equal(a.words.cpu(), b.words)
+    for bad in ((_i32(n), _i32(0)), (_i32(-1), _i32(0)), (_i32(0), _i32(2 * bs))):
+        kv_int4.commit_tree_kv_int4(tk, tv, k, v, *bad)
+        with pytest.raises(RuntimeError, match="out-of-range"):
+            check_status(torch.device(DEV))
+    for a, b in zip((k, v), want):
+        assert torch.equal(a.codes.cpu(), b.codes) and torch.equal(a.words.cpu(), b.words)
+    for bad in ((nodes.long(), slots), (nodes, slots.cpu()), (nodes[:2], slots)):
+        with pytest.raises((RuntimeError, ValueError)):
+            kv_int4.commit_tree_kv_int4(tk, tv, k, v, *bad)
+
+
+@pytest.mark.parametrize("planes", [0, 3])
+@pytest.mark.parametrize("nh,nkv,hd,bs,prefix,nodes", [(8, 2, 128, 32, 77, 6), (14, 2, 64, 16, 300, 10), (4, 4, 128, 64, 5, 10)])
+def test_nodes_are_attended_and_committed_as_decode_stores_them(nh, nkv, hd, bs, prefix, nodes, planes):
+    topo = build_fixed_tree_topology(nodes)
+    n = len(topo.parents)
+    g = torch.Generator().manual_seed(prefix)
+    pools = [oracle.random_pages(-(-(prefix + 4) // bs) + 1, nkv, bs, hd, s) for s in (1, 2)]
+    table = torch.randperm(pools[0][0].shape[0], generator=g)[:-(-(prefix + 4) // bs)].int()
+    wide = (nh + 2 * nkv) * hd
+    qkv = torch.randn(planes, n, wide, generator=g) if planes else torch.randn(n, wide, generator=g).bfloat16()
+    qkv = qkv.to(DEV)
+    norm = [(1 + 0.2 * torch.randn(hd, generator=g)).bfloat16().to(DEV) for _ in range(2)]
+    cos_sin = rope.build_cos_sin_cache(hd, 512, 1e4).to(DEV)
+    positions = torch.tensor([prefix + d for d in topo.depths], device=DEV)
+    layer = Attention(nh, hd, hd ** -0.5, nkv)
+    tree = [Int4Pages(p.codes[None].clone(), p.words[None].clone()) for p in map(_on, pools)]
+    layer.k_cache, layer.v_cache = (p[0] for p in tree)
+    set_context(True, tree_attention_mask=topo.attention_mask(DEV), tree_prefix_len=prefix, tree_block_table=table.to(DEV))
+    got = layer(qkv, positions, cos_sin, *norm, 1e-6).view(n, nh, hd)
+    reset_context()
+
+    # every node as one decoded token: its row of the projection through the decode path's store
+    scratch = [Int4Pages.zeros((n, nkv, 16, hd), DEV) for _ in range(2)]
+    q = kv_int4.qkv_norm_rope_store_int4(qkv, positions, cos_sin, *norm, 1e-6, *scratch,
+                                         torch.arange(n, dtype=torch.int32, device=DEV) * 16, nh, nkv, hd)
+    for node in range(n):
+        # prefix and ancestors in the pages, the way decode would have left them
+        path = topo.ancestors_and_self(node)
+        kp, vp = ((c.clone(), w.clone()) for c, w in pools)
+        for j, a in enumerate(sorted(path, key=lambda x: topo.depths[x])):
+            at = table[(prefix + j) // bs], slice(None), (prefix + j) % bs
+            for p, s in ((kp, scratch[0]), (vp, scratch[1])):
+                p[0][at], p[1][at] = s.codes[a, :, 0].cpu(), s.words[a, :, 0].cpu()
+        keys = prefix + len(path)
+        want, mag = oracle.attention(q[node:node + 1], kp, vp, [0, 1], [keys], table[None], hd ** -0.5)
+        off = (got[node:node + 1].double().cpu() - want).abs()
+        assert (off <= oracle.attention_tolerance(want, mag)).all()
+
+    leaf = max(range(n), key=lambda x: topo.depths[x])
+    path = sorted(topo.ancestors_and_self(leaf), key=lambda x: topo.depths[x])
+    slots = torch.tensor([int(table[(prefix + j) // bs]) * bs + (prefix + j) % bs for j in range(len(path))],
+                         dtype=torch.int32, device=DEV)
+    TreeKVCacheManager([layer], k_cache=tree[0], v_cache=tree[1]).commit(path, slots)
+    for p, s in zip(tree, scratch):
+        for j, a in enumerate(path):
+            at = 0, int(slots[j]) // bs, slice(None), int(slots[j]) % bs
+            assert torch.equal(p.codes[at], s.codes[a, :, 0]) and torch.equal(p.words[at], s.words[a, :, 0])
