@@ -81,6 +81,8 @@ void store_kvcache_int4(at::Tensor k, at::Tensor v, at::Tensor kc, at::Tensor kw
                         at::Tensor slots, at::Tensor status);
 std::tuple<at::Tensor, at::Tensor> load_kvcache_int4(at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                                                      at::Tensor slots, at::Tensor status);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> load_pages_int4(at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                                                               at::Tensor ids);
 void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,
                    at::Tensor k_w, double eps, at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
                    at::Tensor slots, int64_t nh, at::Tensor status);
@@ -145,6 +147,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("feed_ids", &lsb::feed_ids);
   m.def("store_kvcache_int4", &lsb::store_kvcache_int4);
   m.def("load_kvcache_int4", &lsb::load_kvcache_int4);
+  m.def("load_pages_int4", &lsb::load_pages_int4);
   m.def("qkv_rope_int4", &lsb::qkv_rope_int4);
   m.def("prefill_attention_int4", &lsb::prefill_attention_int4);
   m.def("decode_attention_int4", &lsb::decode_attention_int4);

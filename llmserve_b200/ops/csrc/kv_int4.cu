@@ -183,6 +183,34 @@ __global__ void __launch_bounds__(kThreads) load_int4_kernel(
   reinterpret_cast<uint4*>(v)[(size_t)th * kLanes + lane] = dequantise8(cv, wv);
 }
 
+// Whole pages in the layout of a bf16 pool, [n, nkv, bs, HD], and the table that addresses them: i for page i, -1
+// where its id lies outside the pool (its rows are zeros), so that the reader skips and records it.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) load_pages_int4_kernel(
+    bf16* __restrict__ k, bf16* __restrict__ v, int* __restrict__ table, const uint8_t* __restrict__ kc,
+    const int16_t* __restrict__ kw, const uint8_t* __restrict__ vc, const int16_t* __restrict__ vw,
+    const int* __restrict__ ids, uint32_t rows, uint32_t page_rows, uint32_t nblk) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int kLanes = HD / 8;
+  const uint32_t th = blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  if (th >= rows) return;
+  const uint32_t page = th / page_rows, in_page = th - page * page_rows;
+  const uint32_t blk = (uint32_t)ids[page];
+  const bool there = blk < nblk;
+  if (in_page == 0 && lane == 0) table[page] = there ? (int)page : -1;
+  uint32_t ck = 0, cv = 0, wk = 0, wv = 0;         // scale 0: zeros
+  if (there) {
+    const size_t row = (size_t)blk * page_rows + in_page;
+    ck = reinterpret_cast<const uint32_t*>(kc + row * (HD / 2))[lane];
+    cv = reinterpret_cast<const uint32_t*>(vc + row * (HD / 2))[lane];
+    wk = (uint16_t)kw[row * (HD / kGroup) + lane / 8];
+    wv = (uint16_t)vw[row * (HD / kGroup) + lane / 8];
+  }
+  reinterpret_cast<uint4*>(k)[(size_t)th * kLanes + lane] = dequantise8(ck, wk);
+  reinterpret_cast<uint4*>(v)[(size_t)th * kLanes + lane] = dequantise8(cv, wv);
+}
+
 // One step's projection rows [T, (nh + 2 nkv) * HD] (bf16, or S fp32 split-K planes that are summed
 // here): per-head RMS norm of q and k (optional), rotation, q out as bf16, k and v into the pages.
 // Everything between the load and the one rounding at the end is fp32.  HD / 8 lanes hold a head;
@@ -385,6 +413,31 @@ std::tuple<at::Tensor, at::Tensor> load_kvcache_int4(at::Tensor kc, at::Tensor k
   else go(load_int4_kernel<64>);
   launch_check("load_kvcache_int4");
   return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> load_pages_int4(at::Tensor kc, at::Tensor kw, at::Tensor vc, at::Tensor vw,
+                                                               at::Tensor ids) {
+  const at::Device dev = kc.device();
+  check_page_pair(kc, kw, vc, vw, dev);
+  check_int32(ids, "block_table", 1, dev);
+  const int64_t hd = kc.size(3) * 2, page_rows = kc.size(1) * kc.size(2), rows = ids.size(0) * page_rows;
+  LSB_INT4_CHECK(rows < INT32_MAX, "too many rows for one launch");
+  const at::cuda::CUDAGuard g(dev);
+  at::Tensor k = at::empty({ids.size(0), kc.size(1), kc.size(2), hd}, kc.options().dtype(at::kBFloat16)),
+             v = at::empty_like(k), table = at::empty_like(ids);
+  if (rows == 0) return {k, v, table};
+  const int64_t per = kThreads / (hd / 8);
+  const dim3 grid((unsigned)((rows + per - 1) / per));
+  auto go = [&](auto kern) {
+    launch_pdl(kern, grid, dim3(kThreads), 0, at::cuda::getCurrentCUDAStream(), (bf16*)k.data_ptr(),
+               (bf16*)v.data_ptr(), table.data_ptr<int>(), kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>(),
+               vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>(), ids.data_ptr<int>(), (uint32_t)rows, (uint32_t)page_rows,
+               (uint32_t)kc.size(0));
+  };
+  if (hd == 128) go(load_pages_int4_kernel<128>);
+  else go(load_pages_int4_kernel<64>);
+  launch_check("load_pages_int4");
+  return {k, v, table};
 }
 
 void qkv_rope_int4(at::Tensor q_out, at::Tensor qkv, at::Tensor positions, at::Tensor cos_sin, at::Tensor q_w,

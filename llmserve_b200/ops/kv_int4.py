@@ -253,14 +253,15 @@ def tree_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table, 
     given: a node stands for the token that decode would write and read back, so its rows have to be
     what pages hold of them (``qkv_norm_rope_store_int4`` into scratch pages, then ``load_kvcache_int4``)."""
     bs = k_pages.shape[2]
-    n = max(1, -(-prefix_len // bs))
+    prefix_len = min(prefix_len, block_table.shape[0] * bs)      # a context ends at its table
+    ids = block_table[:max(1, -(-prefix_len // bs))]
     if not q.is_cuda:
-        ids = block_table[:n].long()
+        ids = ids.long()
         k, v = (dequantise_int4_ref(p.codes[ids], p.words[ids]).to(q.dtype) for p in (k_pages, v_pages))
+        table = torch.arange(ids.shape[0], dtype=torch.int32)
     else:
-        slots = (block_table[:n].to(torch.int32)[:, None] * bs + torch.arange(bs, dtype=torch.int32, device=q.device)).flatten()
-        k, v = (x.unflatten(0, (-1, bs)).transpose(1, 2).contiguous() for x in load_kvcache_int4(k_pages, v_pages, slots))
-    table = torch.arange(n, dtype=torch.int32, device=q.device)
+        ids = ids.to(torch.int32).contiguous() if ids.shape[0] else torch.full((1,), -1, dtype=torch.int32, device=q.device)
+        k, v, table = C().load_pages_int4(k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, ids)
     return attn_ops.tree_attention(q, k, v, table, prefix_len, tree_k, tree_v, tree_mask, scale, mask_bits)
 
 

@@ -103,3 +103,48 @@ def test_nodes_are_attended_and_committed_as_decode_stores_them(nh, nkv, hd, bs,
         for j, a in enumerate(path):
             at = 0, int(slots[j]) // bs, slice(None), int(slots[j]) % bs
             assert torch.equal(p.codes[at], s.codes[a, :, 0]) and torch.equal(p.words[at], s.words[a, :, 0])
+
+
+def _tree_case(nh, nkv, hd, bs, prefix, n, seed):
+    """(inputs of the operator without the table, 64-bit result for a table of block ids)."""
+    g = torch.Generator().manual_seed(seed)
+    kp, vp = (oracle.random_pages(6, nkv, bs, hd, s) for s in (1, 2))
+    q, tk, tv = (torch.randn(n, h, hd, generator=g).bfloat16() for h in (nh, nkv, nkv))
+    mask = torch.tril(torch.ones(n, n, dtype=torch.bool))
+
+    def want(table):
+        ok = ((table >= 0) & (table < 6)).repeat_interleave(bs)[:prefix]
+        rows = [oracle.values(*p)[table.clamp(0, 5).long()].transpose(1, 2).reshape(-1, nkv, hd)[:prefix][ok] for p in (kp, vp)]
+        k, v = (torch.cat((a, b.double())) for a, b in zip(rows, (tk, tv)))
+        sees = torch.cat((torch.ones(n, int(ok.sum()), dtype=torch.bool), mask), 1)
+        out, mag = torch.zeros(2, n, nh, hd, dtype=torch.float64)
+        for h in range(nh):
+            a = torch.softmax((q[:, h].double() @ k[:, h // (nh // nkv)].T * hd ** -0.5).masked_fill(~sees, -torch.inf), -1)
+            out[:, h], mag[:, h] = a @ v[:, h // (nh // nkv)], a @ v[:, h // (nh // nkv)].abs()
+        return out, mag
+
+    return (q.to(DEV), _on(kp), _on(vp)), (tk.to(DEV), tv.to(DEV), mask.to(DEV), hd ** -0.5), want
+
+
+@pytest.mark.parametrize("nh,nkv,hd,bs", [(8, 2, 128, 32), (14, 2, 64, 48)])         # tensor-core and CUDA-core kernel
+def test_blocks_outside_the_pool_are_not_seen_by_a_tree(nh, nkv, hd, bs):
+    prefix = 5 * bs - 3
+    left, right, want = _tree_case(nh, nkv, hd, bs, prefix, 6, 8)
+    # the last but one: id * block_size passes 2^32 and would wrap to a slot of the pool in 32 bits
+    for bad in (-1, 6, 2 ** 32 // bs + 1, -2 ** 31):
+        table = torch.tensor([4, 1, bad, 0, 3], dtype=torch.int32)
+        out = kv_int4.tree_attention_int4(*left, table.to(DEV), prefix, *right)
+        with pytest.raises(RuntimeError, match="out-of-range"):
+            check_status(torch.device(DEV))
+        ref, mag = want(table)
+        assert ((out.double().cpu() - ref).abs() <= oracle.attention_tolerance(ref, mag)).all()
+
+
+@pytest.mark.parametrize("prefix,blocks", [(0, 0), (0, 2), (1, 1), (64, 2), (200, 3)])
+def test_tree_prefix_ends_at_its_table(prefix, blocks):
+    bs = 32
+    left, right, want = _tree_case(8, 2, 128, bs, min(prefix, blocks * bs), 10, prefix)
+    table = torch.tensor([5, 2, 0][:blocks], dtype=torch.int32)
+    out = kv_int4.tree_attention_int4(*left, table.to(DEV), prefix, *right)
+    ref, mag = want(table)
+    assert ((out.double().cpu() - ref).abs() <= oracle.attention_tolerance(ref, mag)).all()
