@@ -546,6 +546,8 @@ class ModelRunner:
         a[:n], a[n:2 * n] = q_lens, k_lens
         at = 2 * n
         for s, m in zip(seqs, blocks):
+            if len(s.block_table) < m:         # one id would be broadcast over all m places
+                raise IndexError(f"sequence {s.seq_id} holds {len(s.block_table)} blocks, its step needs {m}")
             a[at:at + m] = s.block_table[:m]
             at += m
         self.h2d_bytes += a.nbytes
