@@ -539,12 +539,13 @@ class ModelRunner:
 
     def _device_maps(self, seqs, q_lens: list[int], k_lens: list[int]):
         """The step's maps built on the GPU: one copy of lengths and block ids, one kernel.  Returns
-        ``(maps, key lengths)``."""
+        ``(maps, key lengths, cumulative key lengths)``."""
         bsz, n = self.block_size, len(seqs)
         blocks = [-(-k // bsz) for k in k_lens]
-        a = np.empty(2 * n + sum(blocks), dtype=np.int32)
-        a[:n], a[n:2 * n] = q_lens, k_lens
-        at = 2 * n
+        a = np.empty(3 * n + 1 + sum(blocks), dtype=np.int32)
+        a[:n], a[n:2 * n], a[2 * n] = q_lens, k_lens, 0
+        np.cumsum(k_lens, out=a[2 * n + 1:3 * n + 1])
+        at = 3 * n + 1
         for s, m in zip(seqs, blocks):
             if len(s.block_table) < m:         # one id would be broadcast over all m places
                 raise IndexError(f"sequence {s.seq_id} holds {len(s.block_table)} blocks, its step needs {m}")
@@ -552,8 +553,8 @@ class ModelRunner:
             at += m
         self.h2d_bytes += a.nbytes
         t = _to_device(a, torch.int32, self.device)
-        maps = step_maps.build_step_maps(t[:n], t[n:2 * n], t[2 * n:], bsz, sum(q_lens), max(1, max(blocks)))
-        return maps, t[n:2 * n]
+        maps = step_maps.build_step_maps(t[:n], t[n:2 * n], t[3 * n + 1:], bsz, sum(q_lens), max(1, max(blocks)))
+        return maps, t[n:2 * n], t[2 * n:3 * n + 1]
 
     def prepare_prefill(self, seqs: list[Sequence], decode_seqs: list[Sequence] | None = None):
         decode_ids = {s.seq_id for s in (decode_seqs or [])}
@@ -574,8 +575,8 @@ class ModelRunner:
                 self.check_bounds([s], np.arange(start, end), self._slots(s, start, end))
         if self.is_cuda and len(seqs) <= step_maps.MAX_REQUESTS:
             self.h2d_bytes += 8 * len(ids)
-            maps, seqlens_k = self._device_maps(seqs, q_lens, lens_k)
-            set_context(True, cu_seqlens_q=maps.cu_seqlens_q, max_seqlen_q=max_q, max_seqlen_k=max_k,
+            maps, seqlens_k, cu_k = self._device_maps(seqs, q_lens, lens_k)
+            set_context(True, cu_seqlens_q=maps.cu_seqlens_q, cu_seqlens_k=cu_k, max_seqlen_q=max_q, max_seqlen_k=max_k,
                         slot_mapping=maps.slot_mapping, block_tables=maps.block_tables, seqlens_k=seqlens_k,
                         last_token_indices=maps.last_token_indices, decode_workspace=self.decode_workspace)
             return _to_device(ids, torch.int64, d), maps.positions
@@ -610,7 +611,7 @@ class ModelRunner:
             self.check_bounds(seqs, pos, slots)
         if self.is_cuda and n <= step_maps.MAX_REQUESTS:
             self.h2d_bytes += ids.nbytes
-            maps, context_lens = self._device_maps(seqs, [1] * n, lens.tolist())
+            maps, context_lens, _ = self._device_maps(seqs, [1] * n, lens.tolist())
             set_context(False, slot_mapping=maps.slot_mapping, context_lens=context_lens, block_tables=maps.block_tables,
                         decode_workspace=self.decode_workspace)
             return _to_device(ids, torch.int64, d), maps.positions
