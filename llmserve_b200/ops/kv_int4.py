@@ -233,8 +233,9 @@ def verify_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table
     cap = block_tables.shape[-1] * k_pages.codes.shape[2]
     if workspace is None or workspace.max_batch < rows or workspace.max_splits * 128 < cap:
         workspace = attn_ops.DecodeWorkspace(rows, nh, hd, cap, q.device)
+    q = q.contiguous()
     out = torch.empty_like(q)
-    C().decode_attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, nq,
+    C().decode_attention_int4(out, q, k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, nq,
                               seqlens_k, block_tables, scale, workspace.partial_out, workspace.partial_ml,
                               workspace.counters, workspace.max_splits, status(q.device))
     return out
@@ -262,7 +263,7 @@ def tree_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, block_table, 
     else:
         ids = ids.to(torch.int32).contiguous() if ids.shape[0] else torch.full((1,), -1, dtype=torch.int32, device=q.device)
         k, v, table = C().load_pages_int4(k_pages.codes, k_pages.words, v_pages.codes, v_pages.words, ids)
-    return attn_ops.tree_attention(q, k, v, table, prefix_len, tree_k, tree_v, tree_mask, scale, mask_bits)
+    return attn_ops.tree_attention(q.contiguous(), k, v, table, prefix_len, tree_k, tree_v, tree_mask, scale, mask_bits)
 
 
 def commit_tree_kv_int4(tree_k: Int4Pages, tree_v: Int4Pages, k_pages: Int4Pages, v_pages: Int4Pages, node_indices,
@@ -297,7 +298,8 @@ def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens
     if not q.is_cuda:
         _check_query(q, k_pages, v_pages, scale)
         return attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_tables, scale)
+    q = q.contiguous()
     out = torch.empty_like(q)
-    C().prefill_attention_int4(out, q.contiguous(), k_pages.codes, k_pages.words, v_pages.codes, v_pages.words,
+    C().prefill_attention_int4(out, q, k_pages.codes, k_pages.words, v_pages.codes, v_pages.words,
                                cu_seqlens_q, seqlens_k, block_tables, scale, max_seqlen_q, status(q.device))
     return out

@@ -1,0 +1,58 @@
+"""4-bit KV cache kernels on the calls that their documentation allows beside the ordinary ones."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from llmserve_b200.ops import kv_int4  # noqa: E402
+from llmserve_b200.ops._ext import C, check_status  # noqa: E402
+from llmserve_b200.ops.kv_int4 import Int4Pages  # noqa: E402
+from tests import int4_oracle as oracle  # noqa: E402
+
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    C()
+    yield
+    check_status(torch.device(DEV))
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _on(p):
+    return Int4Pages(p[0].to(DEV), p[1].to(DEV))
+
+
+def _assert_close(got, want, mag):
+    off = (got.double().cpu() - want).abs()
+    tol = oracle.attention_tolerance(want, mag)
+    assert torch.isfinite(got.float()).all()
+    assert (off <= tol).all(), f"{(off / tol).max().item():.3f} of the tolerance"
+
+
+def test_queries_in_any_order_of_strides():
+    """A transposed [heads, rows, head_dim] query is dense but not contiguous; a slice of a wider row is neither."""
+    nh, nkv, hd, bs = 8, 2, 64, 16
+    kp, vp = (oracle.random_pages(6, nkv, bs, hd, s) for s in (1, 2))
+    tables, lens = torch.tensor([[3, 1, 5], [0, 2, 4]], dtype=torch.int32), [41, 30]
+    g = torch.Generator().manual_seed(4)
+    dense = torch.randn(nh, 4, hd, generator=g).bfloat16().to(DEV).transpose(0, 1)
+    wide = torch.randn(4, nh + 2, hd + 64, generator=g).bfloat16().to(DEV)[:, 1:nh + 1, :hd]
+    for q in (dense, wide):
+        assert not q.is_contiguous()
+        args = (q, _on(kp), _on(vp))
+        want, mag = oracle.attention(q, kp, vp, [0, 2, 4], lens, tables, 0.125)
+        _assert_close(kv_int4.verify_attention_int4(*args, tables.to(DEV), _i32(*lens), 0.125, 2), want, mag)
+        _assert_close(kv_int4.prefill_attention_int4(*args, _i32(0, 2, 4), _i32(*lens), tables.to(DEV), 0.125, 2), want, mag)
+        want, mag = oracle.attention(q[:2], kp, vp, [0, 1, 2], lens, tables, 0.125)
+        _assert_close(kv_int4.decode_attention_int4(q[:2], *args[1:], tables.to(DEV), _i32(*lens), 0.125), want, mag)
+        # a tree of two nodes that see themselves, one after the other
+        tk, tv = (torch.randn(2, nkv, hd, generator=g).bfloat16().to(DEV) for _ in range(2))
+        mask = torch.tril(torch.ones(2, 2, dtype=torch.bool, device=DEV))
+        tree = [kv_int4.tree_attention_int4(x, *args[1:], tables[0].to(DEV), 41, tk, tv, mask, 0.125)
+                for x in (q[:2], q[:2].contiguous())]
+        assert torch.equal(*tree) and tree[0].is_contiguous()
