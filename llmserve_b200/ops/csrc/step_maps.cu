@@ -21,26 +21,34 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = 8192;        // 64 KiB of prefix sums in shared memory
 
-// Inclusive block-wide scan of a pair; returns the exclusive prefix and, through `total`, the sum.
+// Sum of two counts (not negative) that stays at INT32_MAX once it gets there: sums of any lengths are in order, and one
+// past int32 is past every limit.
+__device__ __forceinline__ int2 add_sat(int2 a, int2 b) {
+  return make_int2((int)min((uint32_t)a.x + (uint32_t)b.x, (uint32_t)INT32_MAX),
+                   (int)min((uint32_t)a.y + (uint32_t)b.y, (uint32_t)INT32_MAX));
+}
+
+// Block-wide scan of pairs: the sum of the threads before this one and, through `total`, of all.
 __device__ __forceinline__ int2 block_scan(int2 v, int2* scratch, int2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int2 s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
-    if (lane >= o) s.x += a, s.y += b;
+    if (lane >= o) s = add_sat(s, make_int2(a, b));
   }
   __syncthreads();
   if (lane == 31) scratch[warp] = s;
   __syncthreads();
-  int2 before = make_int2(0, 0);
+  int2 before = make_int2(__shfl_up_sync(0xffffffffu, s.x, 1), __shfl_up_sync(0xffffffffu, s.y, 1));
+  if (lane == 0) before = make_int2(0, 0);
   total = make_int2(0, 0);
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before.x += scratch[w].x, before.y += scratch[w].y;
-    total.x += scratch[w].x, total.y += scratch[w].y;
+    if (w < warp) before = add_sat(before, scratch[w]);
+    total = add_sat(total, scratch[w]);
   }
-  return make_int2(before.x + s.x - v.x, before.y + s.y - v.y);
+  return before;
 }
 
 __global__ void __launch_bounds__(kThreads) step_maps_kernel(
@@ -49,31 +57,33 @@ __global__ void __launch_bounds__(kThreads) step_maps_kernel(
     int* __restrict__ tables, int64_t* __restrict__ last, int* status) {
   extern __shared__ int2 first[];          // [B + 1]: (first token, first block id) of each request
   __shared__ int2 scratch[kThreads / 32];
+  __shared__ int first_bad;                // requests from the first contradicting one on count as empty
   pdl_trigger();
   pdl_wait();
+  if (threadIdx.x == 0) first_bad = B;
+  __syncthreads();
   const int per = (B + kThreads - 1) / kThreads, lo = min(B, (int)threadIdx.x * per), hi = min(B, lo + per);
-  bool bad = false;
-  auto lengths = [&](int i) {              // (new tokens, blocks) of request i; a bad one counts as empty
+  for (int i = lo; i < hi; ++i) {
     const int q = q_lens[i], k = k_lens[i];
     if (q < 0 || k < q || q > T) {
-      bad = true;
-      return make_int2(0, 0);
+      atomicMin(&first_bad, i);
+      break;
     }
-    return make_int2(q, (int)(((int64_t)k + bs - 1) / bs));
+  }
+  __syncthreads();
+  const int good = first_bad;
+  auto lengths = [&](int i) {              // (new tokens, blocks) of request i
+    return i < good ? make_int2(q_lens[i], (int)(((int64_t)k_lens[i] + bs - 1) / bs)) : make_int2(0, 0);
   };
   int2 mine = make_int2(0, 0), total;
-  for (int i = lo; i < hi; ++i) {
-    const int2 n = lengths(i);
-    mine.x += n.x, mine.y += n.y;
-  }
+  for (int i = lo; i < hi; ++i) mine = add_sat(mine, lengths(i));
   int2 at = block_scan(mine, scratch, total);
   for (int i = lo; i < hi; ++i) {
     first[i] = at;
-    const int2 n = lengths(i);
-    at.x += n.x, at.y += n.y;
+    at = add_sat(at, lengths(i));
   }
   if (threadIdx.x == 0) first[B] = total;
-  if (blockIdx.x == 0 && (bad || total.x > T || total.y > num_ids)) record_error(status, kBadIndex);
+  if (blockIdx.x == 0 && (good < B || total.x > T || total.y > num_ids)) record_error(status, kBadIndex);
   __syncthreads();
   const int stride = gridDim.x * kThreads, start = blockIdx.x * kThreads + threadIdx.x;
   for (int t = start; t < T; t += stride) {
@@ -86,11 +96,10 @@ __global__ void __launch_bounds__(kThreads) step_maps_kernel(
         if (first[m].x <= t) a = m;
         else b = m;
       }
-      const int p = k_lens[a] - (first[a + 1].x - first[a].x) + (t - first[a].x);
-      const int j = first[a].y + p / bs;
+      const int p = k_lens[a] - q_lens[a] + (t - first[a].x);
       pos = p;
-      if (j >= 0 && j < num_ids) {         // lengths that overflow the sums must not leave the id list either
-        const int64_t s = (int64_t)ids[j] * bs + p % bs;
+      if (p / bs < num_ids - first[a].y) {         // more blocks than ids: the list ends before the sums do
+        const int64_t s = (int64_t)ids[first[a].y + p / bs] * bs + p % bs;
         slot = s >= 0 && s <= INT32_MAX ? (int)s : -1;
       }
     }
@@ -98,9 +107,8 @@ __global__ void __launch_bounds__(kThreads) step_maps_kernel(
     slots[t] = slot;
   }
   for (int i = start; i < B * width; i += stride) {
-    const int row = i / width, j = first[row].y + (i - row * width);
-    const bool in = j >= 0 && j < first[row + 1].y && j < num_ids;
-    tables[i] = in ? ids[j] : 0;
+    const int row = i / width, c = i - row * width, at_row = first[row].y;
+    tables[i] = c < min(first[row + 1].y, num_ids) - at_row ? ids[at_row + c] : 0;
   }
   for (int i = start; i <= B; i += stride) {
     cu[i] = min(first[i].x, T);
@@ -126,7 +134,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_maps
   LSB_INT4_CHECK(bs >= 1 && bs <= INT32_MAX, "block_size must be positive");
   LSB_INT4_CHECK(T >= 0 && width >= 0, "num_tokens and table_width must not be negative");
   LSB_INT4_CHECK(B <= kMaxRequests, "more than 8192 requests in one step");
-  LSB_INT4_CHECK(T <= INT32_MAX - (1 << 20) && B * width <= INT32_MAX - (1 << 20) && ids.size(0) <= INT32_MAX,
+  LSB_INT4_CHECK(T <= INT32_MAX - (1 << 20) && B * width <= INT32_MAX - (1 << 20) && ids.size(0) < INT32_MAX,
                  "step maps exceed int32");
   const at::cuda::CUDAGuard g(dev);
   const auto i32 = q_lens.options(), i64 = i32.dtype(at::kLong);

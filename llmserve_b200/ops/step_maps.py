@@ -62,7 +62,9 @@ def build_step_maps(q_lens: torch.Tensor, k_lens: torch.Tensor, block_ids: torch
     slot -1 (padding of a captured step).  A table row holds its first ``table_width`` ids.  The last
     row of a request without new tokens is the one before its place (0 for the first).  On CUDA,
     lengths that contradict one another (or the ids and rows given) are recorded as an out-of-range
-    index for ``check_status`` and the rows concerned get slot -1."""
+    index for ``check_status``: from the first request with a negative length, more new tokens than keys
+    or more of them than ``num_tokens`` on, requests count as empty (their rows get slot -1), and a row whose block id
+    is not given gets slot -1."""
     if not q_lens.is_cuda:
         _check(q_lens, k_lens, block_ids, block_size, num_tokens, table_width)
         return build_step_maps_ref(q_lens, k_lens, block_ids, block_size, num_tokens, table_width)

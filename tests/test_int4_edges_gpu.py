@@ -4,7 +4,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from llmserve_b200.ops import kv_int4  # noqa: E402
+from llmserve_b200.ops import kv_int4, step_maps  # noqa: E402
 from llmserve_b200.ops._ext import C, check_status  # noqa: E402
 from llmserve_b200.ops.kv_int4 import Int4Pages  # noqa: E402
 from tests import int4_oracle as oracle  # noqa: E402
@@ -56,3 +56,35 @@ def test_queries_in_any_order_of_strides():
         tree = [kv_int4.tree_attention_int4(x, *args[1:], tables[0].to(DEV), 41, tk, tv, mask, 0.125)
                 for x in (q[:2], q[:2].contiguous())]
         assert torch.equal(*tree) and tree[0].is_contiguous()
+
+
+def _recorded():
+    with pytest.raises(RuntimeError, match="out-of-range"):
+        check_status(torch.device(DEV))
+
+
+def test_step_maps_after_a_contradicting_request():
+    """Requests before it are mapped; from it on none is, so that no token lands in another request's block."""
+    for q, k in ((3, 1), (-1, 4), (9, 9)):          # more new tokens than keys, a negative length, more than all rows
+        m = step_maps.build_step_maps(_i32(2, q, 2), _i32(18, k, 2), _i32(4, 5, 6, 7), 16, 8, 3)
+        _recorded()
+        assert m.cu_seqlens_q.tolist() == [0, 2, 2, 2]
+        assert m.slot_mapping.tolist() == [5 * 16, 5 * 16 + 1] + [-1] * 6
+        assert m.positions.tolist() == [16, 17] + [0] * 6
+        assert m.block_tables.tolist() == [[4, 5, 0], [0, 0, 0], [0, 0, 0]]
+
+
+def test_step_maps_of_lengths_whose_sums_pass_32_bits():
+    # blocks: 2 (2^31 - 1) wraps to -2, which no id list is too short for
+    m = step_maps.build_step_maps(_i32(1, 1), _i32(2 ** 31 - 1, 2 ** 31 - 1), _i32(0, 1), 1, 2, 1)
+    _recorded()
+    assert m.slot_mapping.tolist() == [-1, -1] and m.cu_seqlens_q.tolist() == [0, 1, 2]
+    # new tokens: 8192 * 2^18 = 2^31
+    n, t = 8192, 2 ** 18
+    lens = torch.full((n,), t, dtype=torch.int32, device=DEV)
+    ids = torch.arange(n, dtype=torch.int32, device=DEV)
+    m = step_maps.build_step_maps(lens, lens, ids, t, t, 1)
+    _recorded()
+    assert m.cu_seqlens_q.tolist() == [0] + [t] * n and m.last_token_indices.tolist() == [t - 1] * n
+    assert torch.equal(m.slot_mapping, torch.arange(t, dtype=torch.int32, device=DEV))
+    assert torch.equal(m.block_tables.flatten(), ids)
