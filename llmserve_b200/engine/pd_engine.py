@@ -204,7 +204,10 @@ class PDEngine:
 
     def __init__(self, model, **kwargs):
         from llmserve_b200.engine.llm_engine import LLMEngine
-        if kwargs.get("kv_cache_dtype", "auto") != "auto":
+        dtype = kwargs.get("kv_cache_dtype", "auto")
+        if dtype not in ("auto", "int4"):
+            raise ValueError("kv_cache_dtype must be 'auto' or 'int4'")
+        if dtype != "auto":
             raise ValueError("kv_cache_dtype='int4' does not support prefill/decode disaggregation")
         pre = tuple(kwargs.pop("pd_prefill_devices", ()) or ())
         dec = tuple(kwargs.pop("pd_decode_devices", ()) or ())
