@@ -157,7 +157,12 @@ def attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_table
                 for p in (k_pages, v_pages))
         last = torch.arange(lens[i] - (hi - lo), lens[i], device=q.device).unsqueeze(1)
         mask = torch.arange(k_len, device=q.device).unsqueeze(0) <= last
-        o = attn_ops._attend(q[lo:hi], k, v, scale, mask)
+        # a group of V that holds NaN reaches the rows that see its key, not those that give it no weight
+        nan = v.isnan()
+        o = attn_ops._attend(q[lo:hi], k, v.masked_fill(nan, 0), scale, mask)
+        if nan.any():
+            seen = (mask.float() @ nan.flatten(1).float()).view(-1, *nan.shape[1:]) > 0
+            o = o.masked_fill(seen.repeat_interleave(q.shape[1] // k.shape[1], 1), float("nan"))
         out[lo:hi] = torch.where(mask.any(1)[:, None, None], o, torch.zeros_like(o))
     return out
 
