@@ -160,9 +160,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   const int G = nh / nkv, per_tile = kBQ / G;              // queries of a tile
   const int kvh = blockIdx.x % nkv, want = blockIdx.x / nkv;
   int seq = -1, pair = 0, base = 0;
+  auto row_at = [&](int b) { return max(0, min(T, cu_q[b])); };      // first row of sequence b, whatever the table holds
   for (int b0 = 0; b0 < B && seq < 0; b0 += 32) {
     int n = 0;
-    if (b0 + lane < B) n = (max(0, min(cu_q[b0 + lane + 1], T) - max(0, min(T, cu_q[b0 + lane]))) + 2 * per_tile - 1) / (2 * per_tile);
+    if (b0 + lane < B) n = (max(0, row_at(b0 + lane + 1) - row_at(b0 + lane)) + 2 * per_tile - 1) / (2 * per_tile);
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     base += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (seq < 0) return;
-  const int q0 = max(0, min(T, cu_q[seq])), q_len = min(cu_q[seq + 1], T) - q0;
+  const int q0 = row_at(seq), q_len = row_at(seq + 1) - q0;
   const int first = pair * 2 * per_tile;
   const int k_cap = max(0, min(k_lens[seq], (int)min((int64_t)width * bs, (int64_t)INT32_MAX - kBK)));
   const int shift = k_lens[seq] - q_len;                   // absolute position of query 0

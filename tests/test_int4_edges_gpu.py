@@ -88,3 +88,19 @@ def test_step_maps_of_lengths_whose_sums_pass_32_bits():
     assert m.cu_seqlens_q.tolist() == [0] + [t] * n and m.last_token_indices.tolist() == [t - 1] * n
     assert torch.equal(m.slot_mapping, torch.arange(t, dtype=torch.int32, device=DEV))
     assert torch.equal(m.block_tables.flatten(), ids)
+
+
+def test_prefill_takes_row_tables_that_leave_the_query():
+    """Cumulative lengths below zero, past the rows, out of order: rows of the query are worked on, nothing else."""
+    nh, nkv, hd, bs = 4, 2, 64, 16
+    kp, vp = (oracle.random_pages(4, nkv, bs, hd, s) for s in (1, 2))
+    q = torch.randn(5, nh, hd, generator=torch.Generator().manual_seed(7)).bfloat16()
+    tables = torch.tensor([[3, 1], [0, 2], [1, 0]], dtype=torch.int32)
+    args = (q.to(DEV), _on(kp), _on(vp))
+    low = -2 ** 31
+    for given, seen in (((low, 2, 2, low), (0, 2, 2, 2)), ((0, 2, 2 ** 31 - 1, 5), (0, 2, 5, 5)), ((low, low, low, low), (0, 0, 0, 0)),
+                        ((0, 2, 5, low), (0, 2, 5, 5))):
+        out = kv_int4.prefill_attention_int4(*args, _i32(*given), _i32(20, 30, 9), tables.to(DEV), 0.125, 5)
+        want, mag = oracle.attention(q, kp, vp, seen, [20, 30, 9], tables, 0.125)
+        n = seen[-1]
+        _assert_close(out[:n], want[:n], mag[:n])
