@@ -137,8 +137,8 @@ struct TileFlags {
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
     bf16* __restrict__ out, const bf16* __restrict__ q, Pages kp, Pages vp, const int* __restrict__ cu_q,
-    const int* __restrict__ k_lens, const int* __restrict__ tables, int width, int B, int T, float scale_log2, int nh,
-    int nkv, int bs, int nblk, int* __restrict__ status) {
+    const int* __restrict__ k_lens, const int* __restrict__ tables, int width, int B, int T, int max_q, float scale_log2,
+    int nh, int nkv, int bs, int nblk, int* __restrict__ status) {
   using L = PfLayout<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_int4_kernel(
   auto row_at = [&](int b) { return max(0, min(T, cu_q[b])); };      // first row of sequence b, whatever the table holds
   for (int b0 = 0; b0 < B && seq < 0; b0 += 32) {
     int n = 0;
-    if (b0 + lane < B) n = (max(0, row_at(b0 + lane + 1) - row_at(b0 + lane)) + 2 * per_tile - 1) / (2 * per_tile);
+    if (b0 + lane < B) n = (max(0, min(max_q, row_at(b0 + lane + 1) - row_at(b0 + lane))) + 2 * per_tile - 1) / (2 * per_tile);
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -588,8 +588,8 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
                (bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), Pages{kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
                Pages{vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, (const int*)cu_q.data_ptr<int>(),
                (const int*)k_lens.data_ptr<int>(), (const int*)tables.data_ptr<int>(), (int)tables.size(1), (int)B, (int)T,
-               (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs, (int)kc.size(0),
-               status_ptr(status));
+               (int)std::min(max_q, T), (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs,
+               (int)kc.size(0), status_ptr(status));
   };
   if (hd == 128) go(prefill_int4_kernel<128>, PfLayout<128>::kBytes);
   else go(prefill_int4_kernel<64>, PfLayout<64>::kBytes);

@@ -298,8 +298,8 @@ def commit_tree_kv_int4(tree_k: Int4Pages, tree_v: Int4Pages, k_pages: Int4Pages
 def prefill_attention_int4(q, k_pages: Int4Pages, v_pages: Int4Pages, cu_seqlens_q, seqlens_k, block_tables, scale,
                            max_seqlen_q: int):
     """Varlen causal attention of packed query rows ``[T, nh, hd]``; row ``j`` of a chunk of ``q_len``
-    sees keys ``< seqlens_k - q_len + j + 1``.  ``max_seqlen_q`` is at least the longest chunk (rows past
-    it, like rows behind the last sequence, are left unwritten)."""
+    sees keys ``< seqlens_k - q_len + j + 1``.  ``max_seqlen_q`` is at least the longest chunk: of a
+    longer one, rows are left unwritten, as are the rows behind the last sequence."""
     if not q.is_cuda:
         _check_query(q, k_pages, v_pages, scale)
         return attention_int4_ref(q, k_pages, v_pages, cu_seqlens_q, seqlens_k, block_tables, scale)

@@ -104,3 +104,15 @@ def test_prefill_takes_row_tables_that_leave_the_query():
         want, mag = oracle.attention(q, kp, vp, seen, [20, 30, 9], tables, 0.125)
         n = seen[-1]
         _assert_close(out[:n], want[:n], mag[:n])
+
+
+def test_a_chunk_longer_than_stated_costs_no_other_sequence_its_rows():
+    nh, nkv, hd, bs = 64, 2, 64, 16                       # 32 heads a KV head: four queries a tile, eight a block
+    q_lens, k_lens = [90, 3, 7], [90, 20, 7]
+    kp, vp = (oracle.random_pages(9, nkv, bs, hd, s) for s in (1, 2))
+    tables = torch.tensor([[3, 1, 8, 0, 5, 2], [4, 6, 0, 0, 0, 0], [7, 0, 0, 0, 0, 0]], dtype=torch.int32)
+    q = torch.randn(100, nh, hd, generator=torch.Generator().manual_seed(7)).bfloat16()
+    out = kv_int4.prefill_attention_int4(q.to(DEV), _on(kp), _on(vp), _i32(0, 90, 93, 100), _i32(*k_lens), tables.to(DEV), 0.125, 7)
+    want, mag = oracle.attention(q, kp, vp, [0, 90, 93, 100], k_lens, tables, 0.125)
+    _assert_close(out[90:], want[90:], mag[90:])
+    _assert_close(out[:7], want[:7], mag[:7])
