@@ -34,7 +34,6 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <cmath>
 #include <type_traits>
 
 #include "int4_pages.cuh"
@@ -578,7 +577,7 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
   const int64_t B = lens.size(0), T = q.size(0), nh = q.size(1), nkv = kc.size(1), hd = q.size(2), bs = kc.size(2);
   LSB_INT4_CHECK(tables.size(0) >= B, "block_tables must hold one row per sequence");
   LSB_INT4_CHECK(nq >= 1 && T == B * nq, "q must hold nq rows per sequence");
-  LSB_INT4_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
+  const float factor = scale_log2(scale, 16);
   if (T == 0) return;
   const int64_t cap = tables.size(1) * bs;
   LSB_INT4_CHECK(part_o.scalar_type() == at::kFloat && part_ml.scalar_type() == at::kFloat &&
@@ -596,7 +595,7 @@ void decode_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tens
   Args a = {(bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), {kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
             {vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, lens.data_ptr<int>(), tables.data_ptr<int>(),
             part_o.data_ptr<float>(), part_ml.data_ptr<float>(), counters.data_ptr<int>(), status_ptr(status),
-            (float)(scale * 16 * 1.4426950408889634), (int)tables.size(1), (int)B, (int)nq, (int)nh, (int)nkv, (int)bs,
+            factor, (int)tables.size(1), (int)B, (int)nq, (int)nh, (int)nkv, (int)bs,
             (int)kc.size(0), (int)max_splits, tiles, bs == 16 ? 0u : (uint32_t)(((1ll << 32) + bs / 16 - 1) / (bs / 16))};
   auto go = [&](auto kern, int smem) {
     ensure_dynamic_smem((const void*)kern, smem);

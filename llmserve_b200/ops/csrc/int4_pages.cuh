@@ -10,6 +10,8 @@
 #pragma once
 #include <ATen/ATen.h>
 
+#include <cmath>
+
 #include "common.cuh"
 
 namespace lsb {
@@ -54,6 +56,14 @@ inline void check_int32(const at::Tensor& t, const char* name, int64_t dim, cons
   LSB_INT4_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == dev,
                  std::string(name) + " must be contiguous int32 with " + std::to_string(dim) +
                      " dimension(s) on the device of the other arguments");
+}
+
+// What scores are multiplied by, for exponentials of base two: `times` times the scale in float32, which must not
+// round to zero (a hidden score, minus infinity, would become NaN) or to infinity.
+inline float scale_log2(double scale, double times) {
+  const float s = (float)(scale * times * 1.4426950408889634);
+  LSB_INT4_CHECK(s >= 1.17549435e-38f && std::isfinite(s), "scale must be positive and within the range of float32");
+  return s;
 }
 
 }  // namespace int4

@@ -29,8 +29,6 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <cmath>
-
 #include "int4_pages.cuh"
 #include "umma.cuh"
 
@@ -574,7 +572,7 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
   const int64_t B = k_lens.size(0);
   LSB_INT4_CHECK(tables.size(0) >= B, "block_tables must hold one row per sequence");
   LSB_INT4_CHECK(cu_q.size(0) == B + 1, "cu_seqlens_q must hold one entry more than there are sequences");
-  LSB_INT4_CHECK(scale > 0 && std::isfinite(scale), "scale must be positive");
+  const float factor = scale_log2(scale, 1);
   LSB_INT4_CHECK(kc.numel() / (hd / 2) / 16 < INT32_MAX && T < INT32_MAX, "pages exceed int32 rows of 16 keys");
   if (T == 0 || B == 0 || max_q <= 0) return;
   const at::cuda::CUDAGuard guard(dev);
@@ -588,7 +586,7 @@ void prefill_attention_int4(at::Tensor out, at::Tensor q, at::Tensor kc, at::Ten
                (bf16*)out.data_ptr(), (const bf16*)q.data_ptr(), Pages{kc.data_ptr<uint8_t>(), kw.data_ptr<int16_t>()},
                Pages{vc.data_ptr<uint8_t>(), vw.data_ptr<int16_t>()}, (const int*)cu_q.data_ptr<int>(),
                (const int*)k_lens.data_ptr<int>(), (const int*)tables.data_ptr<int>(), (int)tables.size(1), (int)B, (int)T,
-               (int)std::min(max_q, T), (float)(scale * 1.4426950408889634), (int)nh, (int)nkv, (int)bs,
+               (int)std::min(max_q, T), factor, (int)nh, (int)nkv, (int)bs,
                (int)kc.size(0), status_ptr(status));
   };
   if (hd == 128) go(prefill_int4_kernel<128>, PfLayout<128>::kBytes);

@@ -116,3 +116,14 @@ def test_a_chunk_longer_than_stated_costs_no_other_sequence_its_rows():
     want, mag = oracle.attention(q, kp, vp, [0, 90, 93, 100], k_lens, tables, 0.125)
     _assert_close(out[90:], want[90:], mag[90:])
     _assert_close(out[:7], want[:7], mag[:7])
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), float("inf"), 1e-46, 1e39])
+def test_scales_that_float32_does_not_hold_are_refused(scale):
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    p = Int4Pages.zeros((1, 2, 16, 64), DEV)
+    t, n = _i32(0).view(1, 1), _i32(1)
+    with pytest.raises(RuntimeError, match="scale"):
+        kv_int4.decode_attention_int4(q, p, p, t, n, scale)
+    with pytest.raises(RuntimeError, match="scale"):
+        kv_int4.prefill_attention_int4(q, p, p, _i32(0, 1), n, t, scale, 1)
