@@ -64,6 +64,7 @@ void decode_attention_tma(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tenso
                           at::Tensor counters, int64_t max_splits, int64_t partition, int64_t nq,
                           at::Tensor status);
 bool decode_tma_supported(int64_t block_size, int64_t head_dim);
+int64_t kv_pool_map_count();
 bool prefill_tc_supported(int64_t block_size, int64_t head_dim);
 bool tree_tc_supported(int64_t n_q, int64_t nh, int64_t nkv, int64_t n_tree, int64_t block_size, int64_t head_dim);
 void tree_attention_tc(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor vc, at::Tensor bt, int64_t prefix_len,
@@ -116,6 +117,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_bf16_packed", &lsb::gemm_bf16_packed);
   m.def("awq_gemm", &lsb::awq_gemm);
   m.def("decode_tma_supported", &lsb::decode_tma_supported);
+  m.def("kv_pool_map_count", &lsb::kv_pool_map_count);
   m.def("decode_attention", &lsb::decode_attention, py::arg("out"), py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_tables"), py::arg("context_lens"), py::arg("scale"), py::arg("part_o"), py::arg("part_ml"),
         py::arg("counters"), py::arg("max_splits"), py::arg("partition"), py::arg("grid_z"), py::arg("status"));

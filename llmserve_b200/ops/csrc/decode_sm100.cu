@@ -440,15 +440,23 @@ struct PoolKeyHash {
   }
 };
 
-// Tensor map over one layer's K or V pool viewed as [blocks * kv_heads * block_size, head_dim].
-const CUtensorMap& pool_map(const at::Tensor& pool, int box_rows) {
+std::unordered_map<PoolKey, CUtensorMap, PoolKeyHash>& pool_maps() {
   static std::unordered_map<PoolKey, CUtensorMap, PoolKeyHash> cache;
+  return cache;
+}
+// Pools of hundreds of layers, and an end for the copies of 4-bit prefixes, which come with new sizes and addresses.
+constexpr size_t kMaxPoolMaps = 4096;
+
+// Tensor map over one layer's K or V pool viewed as [blocks * kv_heads * block_size, head_dim].
+CUtensorMap pool_map(const at::Tensor& pool, int box_rows) {
   static std::mutex mu;
   const int64_t hd = pool.size(3), rows = pool.numel() / hd;
   PoolKey key{pool.data_ptr(), rows, hd, box_rows};
   std::lock_guard<std::mutex> lock(mu);
+  auto& cache = pool_maps();
   auto it = cache.find(key);
   if (it != cache.end()) return it->second;
+  if (cache.size() >= kMaxPoolMaps) cache.clear();
   CUtensorMap m;
   cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
@@ -475,7 +483,8 @@ int sm_count() {
 
 // Tensor map over one layer's K or V pool viewed as [blocks * kv_heads * block_size, head_dim] with a
 // (box_rows x 64 dims) box, 128B swizzle; cached per (pool, box).  Shared with the prefill kernel.
-const CUtensorMap& kv_pool_map(const at::Tensor& pool, int box_rows) { return pool_map(pool, box_rows); }
+CUtensorMap kv_pool_map(const at::Tensor& pool, int box_rows) { return pool_map(pool, box_rows); }
+int64_t kv_pool_map_count() { return (int64_t)pool_maps().size(); }
 
 // Whether decode_attention_tma supports this pool (block size and head dim).
 bool decode_tma_supported(int64_t block_size, int64_t head_dim) {
@@ -512,8 +521,7 @@ void decode_attention_tma(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tenso
   if (B == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
   const int box_rows = bs >= 64 ? 64 : bs;
-  const CUtensorMap& mk = pool_map(kc, box_rows);
-  const CUtensorMap& mv = pool_map(vc, box_rows);
+  const CUtensorMap mk = pool_map(kc, box_rows), mv = pool_map(vc, box_rows);
   const int64_t n_items = (int64_t)max_chunks * B * nkv;
   const int G = nh / nkv;
   const float sl = (float)scale * kLog2e;

@@ -42,7 +42,7 @@
 namespace lsb {
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
-const CUtensorMap& kv_pool_map(const at::Tensor& pool, int box_rows);
+CUtensorMap kv_pool_map(const at::Tensor& pool, int box_rows);
 int* status_ptr(const at::Tensor& status);
 
 namespace {
@@ -471,8 +471,7 @@ void prefill_attention_tc(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tenso
     LSB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed for q (" + std::to_string((int)r) + ")");
   }
   const int box_keys = bs >= 64 ? 64 : bs;
-  const CUtensorMap& tm_k = kv_pool_map(kc, box_keys);
-  const CUtensorMap& tm_v = kv_pool_map(vc, box_keys);
+  const CUtensorMap tm_k = kv_pool_map(kc, box_keys), tm_v = kv_pool_map(vc, box_keys);
   const int pairs = (int)((max_q + kQTiles * kBQ - 1) / (kQTiles * kBQ));
   LSB_CHECK((int64_t)pairs * B < 65536, "too many query tiles for one launch");
   const float sl = (float)scale * kLog2e;

@@ -39,7 +39,7 @@
 
 namespace lsb {
 
-const CUtensorMap& kv_pool_map(const at::Tensor& pool, int box_rows);
+CUtensorMap kv_pool_map(const at::Tensor& pool, int box_rows);
 int* status_ptr(const at::Tensor& status);
 
 namespace {
@@ -511,8 +511,7 @@ void tree_attention_tc(at::Tensor out, at::Tensor q, at::Tensor kc, at::Tensor v
   float* po = chunks > 1 ? part_o.data_ptr<float>() : nullptr;
   float* pml = chunks > 1 ? part_ml.data_ptr<float>() : nullptr;
   const int box_keys = bs >= 64 ? 64 : bs;
-  const CUtensorMap& tm_k = kv_pool_map(kc, box_keys);
-  const CUtensorMap& tm_v = kv_pool_map(vc, box_keys);
+  const CUtensorMap tm_k = kv_pool_map(kc, box_keys), tm_v = kv_pool_map(vc, box_keys);
   const bf16* tkp = n_tree ? (const bf16*)tk.data_ptr() : nullptr;
   const bf16* tvp = n_tree ? (const bf16*)tv.data_ptr() : nullptr;
   const float sl = (float)scale * kTLog2e;

@@ -148,3 +148,17 @@ def test_tree_prefix_ends_at_its_table(prefix, blocks):
     out = kv_int4.tree_attention_int4(*left, table.to(DEV), prefix, *right)
     ref, mag = want(table)
     assert ((out.double().cpu() - ref).abs() <= oracle.attention_tolerance(ref, mag)).all()
+
+
+def test_prefix_copies_of_ever_new_sizes_keep_no_more_than_a_bounded_set():
+    """Two tensor maps a size: 2200 sizes pass the bound of 4096."""
+    from llmserve_b200.ops._ext import raw_module
+    left, right, want = _tree_case(4, 2, 64, 16, 33, 6, 5)
+    table = torch.tensor([5, 2, 0], dtype=torch.int32)
+    ref, mag = want(table)
+    long = torch.zeros(2200, dtype=torch.int32, device=DEV)
+    for n in range(1, 2200):
+        kv_int4.tree_attention_int4(*left, long, 16 * n, *right)
+        assert raw_module().kv_pool_map_count() <= 4096
+    out = kv_int4.tree_attention_int4(*left, table.to(DEV), 33, *right)
+    assert ((out.double().cpu() - ref).abs() <= oracle.attention_tolerance(ref, mag)).all()
