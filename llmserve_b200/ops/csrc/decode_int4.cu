@@ -71,11 +71,6 @@ struct DecLayout {
   static constexpr int kBytes = kBarOff + kWarps * kStages * 8;
 };
 
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -92,11 +87,6 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t x, uint32_t m, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(z));
   return y;
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t x, uint32_t m) {
-  uint32_t y;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(m));
-  return y;
-}
 // The patterns 0 .. 255 of bf16 (subnormals and the first binade) are one even grid: n 2^-133.  So a nibble
 // masked where it stands is c 2^-133 or, four bits up, c 2^-129, and one multiply-add by 2^127 makes the
 // exact (c - z) / 64 or (c - z) / 4.
@@ -106,8 +96,8 @@ struct Zeros {
   uint32_t low, high;
 };
 __device__ __forceinline__ Zeros zeros(uint32_t w) {
-  const uint32_t low = mul_bf16x2(w & 0x000f000fu, kUp | 0x80008000u);
-  return {low, mul_bf16x2(low, 0x41804180u)};
+  const uint32_t low = mul2(w & 0x000f000fu, kUp | 0x80008000u);
+  return {low, mul2(low, 0x41804180u)};
 }
 // nibbles (s, s + 4) of a word less the lanes' zero codes: /64 for even s, /4 for odd s
 __device__ __forceinline__ void codes_bf16(uint32_t w, const Zeros& z, uint32_t* y) {
@@ -332,10 +322,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_int4_kernel(con
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint4 v = live ? src[(gr * 64 + t4 * 16 + i * 8) / 8] : make_uint4(0, 0, 0, 0);
-          qf[gr][i][0] = mul_bf16x2(__byte_perm(v.x, v.z, 0x5410), 0x40804080u);
-          qf[gr][i][1] = mul_bf16x2(__byte_perm(v.x, v.z, 0x7632), 0x3e803e80u);
-          qf[gr][i][2] = mul_bf16x2(__byte_perm(v.y, v.w, 0x5410), 0x40804080u);
-          qf[gr][i][3] = mul_bf16x2(__byte_perm(v.y, v.w, 0x7632), 0x3e803e80u);
+          qf[gr][i][0] = mul2(__byte_perm(v.x, v.z, 0x5410), 0x40804080u);
+          qf[gr][i][1] = mul2(__byte_perm(v.x, v.z, 0x7632), 0x3e803e80u);
+          qf[gr][i][2] = mul2(__byte_perm(v.y, v.w, 0x5410), 0x40804080u);
+          qf[gr][i][3] = mul2(__byte_perm(v.y, v.w, 0x7632), 0x3e803e80u);
         }
     }
     // keys that row r of the block sees, and keys that all its rows see

@@ -19,6 +19,24 @@ namespace int4 {
 
 constexpr int kGroup = 64;
 
+// a pair of bf16 at a time
+__device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t z) {
+  uint32_t y;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+  return y;
+}
+// global to shared memory, counted by an mbarrier; both addresses and the size are multiples of 16 bytes
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 struct Pages {
   const uint8_t* codes;
   const int16_t* words;

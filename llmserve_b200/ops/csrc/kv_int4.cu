@@ -91,16 +91,6 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* x) {
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ uint32_t sub2(uint32_t x, uint32_t z) {
-  uint32_t y;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
-  return y;
-}
-__device__ __forceinline__ uint32_t mul2(uint32_t x, uint32_t z) {
-  uint32_t y;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
