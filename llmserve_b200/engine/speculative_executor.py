@@ -421,8 +421,8 @@ class SpeculativeExecutor:
 
         t = perf_counter()
         base = len(seq) - (1 if merged else 0)
-        set_context(True, tree_attention_mask=mask, tree_prefix_len=base, tree_block_table=table,
-                    tree_mask_bits=bits)
+        set_context(True, tree_attention_mask=mask, tree_prefix_len=base, tree_block_table=table, tree_mask_bits=bits,
+                    slot_mapping=torch.arange(n_nodes, dtype=torch.int32, device=dev))
         try:
             hidden, aux = r.model.forward_with_eagle3_aux(
                 torch.tensor(tokens, dtype=torch.int64, device=dev),

@@ -72,8 +72,10 @@ class Attention(nn.Module):
         # scratch pages of one block: the kernel that quantises a decoded token's K/V quantises the nodes'
         T = positions.shape[0]
         shape = (1, self.num_kv_heads, -(-T // 16) * 16, self.head_dim)
-        pages = [kv_int4.Int4Pages.zeros(shape, qkv.device) for _ in range(2)]
-        slots = torch.arange(T, dtype=torch.int32, device=qkv.device)
+        pages = [kv_int4.Int4Pages.empty(shape, qkv.device) for _ in range(2)]
+        slots = ctx.slot_mapping             # node i in row i
+        if slots is None:
+            slots = torch.arange(T, dtype=torch.int32, device=qkv.device)
         q = kv_int4.qkv_norm_rope_store_int4(qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, *pages, slots,
                                              self.num_heads, self.num_kv_heads, self.head_dim)
         self.tree_k, self.tree_v = (p.rows(T) for p in pages)

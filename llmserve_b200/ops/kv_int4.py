@@ -36,13 +36,21 @@ class Int4Pages:
         self.codes, self.words = codes, words
 
     @classmethod
-    def zeros(cls, shape, device) -> "Int4Pages":
-        """Empty pages for logical rows ``[..., blocks, kv_heads, block_size, head_dim]``."""
+    def empty(cls, shape, device) -> "Int4Pages":
+        """Pages of any content for logical rows ``[..., blocks, kv_heads, block_size, head_dim]``."""
         *lead, hd = shape
         if hd not in (64, 128) or lead[-1] % 16:
             raise ValueError("4-bit pages need head_dim 64 or 128 and a block_size that is a multiple of 16")
-        return cls(torch.zeros(*lead, hd // 2, dtype=torch.uint8, device=device),
-                   torch.zeros(*lead, hd // GROUP, dtype=torch.int16, device=device))
+        return cls(torch.empty(*lead, hd // 2, dtype=torch.uint8, device=device),
+                   torch.empty(*lead, hd // GROUP, dtype=torch.int16, device=device))
+
+    @classmethod
+    def zeros(cls, shape, device) -> "Int4Pages":
+        """The same, every row zero."""
+        pages = cls.empty(shape, device)
+        pages.codes.zero_()
+        pages.words.zero_()
+        return pages
 
     @property
     def shape(self) -> tuple:
