@@ -69,10 +69,10 @@ class Attention(nn.Module):
                                              self.scale, ctx.decode_workspace)
 
     def _forward_tree_int4(self, qkv, positions, cos_sin, q_norm_w, k_norm_w, eps, ctx) -> torch.Tensor:
-        # scratch pages of one block: the kernel that quantises a decoded token's K/V quantises the nodes'
+        # scratch pages of one block: the kernel that quantises a decoded token's K/V quantises the nodes'.  A node
+        # whose position is outside the angle table is skipped: it reads as zeros, since V that nobody sees has to be finite
         T = positions.shape[0]
-        shape = (1, self.num_kv_heads, -(-T // 16) * 16, self.head_dim)
-        pages = [kv_int4.Int4Pages.empty(shape, qkv.device) for _ in range(2)]
+        pages = kv_int4.Int4Pages.scratch_pair((1, self.num_kv_heads, -(-T // 16) * 16, self.head_dim), qkv.device)
         slots = ctx.slot_mapping             # node i in row i
         if slots is None:
             slots = torch.arange(T, dtype=torch.int32, device=qkv.device)

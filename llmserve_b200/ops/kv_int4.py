@@ -36,21 +36,21 @@ class Int4Pages:
         self.codes, self.words = codes, words
 
     @classmethod
-    def empty(cls, shape, device) -> "Int4Pages":
-        """Pages of any content for logical rows ``[..., blocks, kv_heads, block_size, head_dim]``."""
+    def zeros(cls, shape, device) -> "Int4Pages":
+        """Empty pages for logical rows ``[..., blocks, kv_heads, block_size, head_dim]``."""
         *lead, hd = shape
         if hd not in (64, 128) or lead[-1] % 16:
             raise ValueError("4-bit pages need head_dim 64 or 128 and a block_size that is a multiple of 16")
-        return cls(torch.empty(*lead, hd // 2, dtype=torch.uint8, device=device),
-                   torch.empty(*lead, hd // GROUP, dtype=torch.int16, device=device))
+        return cls(torch.zeros(*lead, hd // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(*lead, hd // GROUP, dtype=torch.int16, device=device))
 
     @classmethod
-    def zeros(cls, shape, device) -> "Int4Pages":
-        """The same, every row zero."""
-        pages = cls.empty(shape, device)
-        pages.codes.zero_()
-        pages.words.zero_()
-        return pages
+    def scratch_pair(cls, shape, device) -> tuple["Int4Pages", "Int4Pages"]:
+        """K and V pages whose rows read as zeros until they are stored (scale 0; the codes hold anything)."""
+        *lead, hd = shape
+        pair = cls(torch.empty(2, *lead, hd // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(2, *lead, hd // GROUP, dtype=torch.int16, device=device))
+        return pair[0], pair[1]
 
     @property
     def shape(self) -> tuple:

@@ -162,3 +162,31 @@ def test_prefix_copies_of_ever_new_sizes_keep_no_more_than_a_bounded_set():
         assert raw_module().kv_pool_map_count() <= 4096
     out = kv_int4.tree_attention_int4(*left, table.to(DEV), 33, *right)
     assert ((out.double().cpu() - ref).abs() <= oracle.attention_tolerance(ref, mag)).all()
+
+
+def test_nodes_past_the_last_position_leave_the_others_as_they_are():
+    """The deepest nodes of a tree at the end of the model's positions are skipped and recorded; scratch memory that
+    held NaN patterns before must not reach the nodes above them."""
+    nh, nkv, hd, bs, prefix = 8, 2, 64, 16, 37
+    topo = build_fixed_tree_topology(10)
+    n = len(topo.parents)
+    g = torch.Generator().manual_seed(2)
+    layer = Attention(nh, hd, hd ** -0.5, nkv)
+    layer.k_cache, layer.v_cache = (_on(oracle.random_pages(3, nkv, bs, hd, s)) for s in (1, 2))
+    qkv = torch.randn(n, (nh + 2 * nkv) * hd, generator=g).bfloat16().to(DEV)
+    positions = torch.tensor([prefix + d for d in topo.depths], device=DEV)
+    weight = torch.ones(hd, dtype=torch.bfloat16, device=DEV)
+    cos_sin = rope.build_cos_sin_cache(hd, 512, 1e4).to(DEV)
+    set_context(True, tree_attention_mask=topo.attention_mask(DEV), tree_prefix_len=prefix, tree_block_table=_i32(2, 0, 1))
+    want = layer(qkv, positions, cos_sin, weight, weight, 1e-6)
+    last = prefix + max(topo.depths)
+    short = cos_sin[:last].contiguous()
+    for _ in range(3):
+        junk = [torch.full((size,), 255, dtype=torch.uint8, device=DEV) for size in (512, 1024, 1088, 2048, 2176, 4096, 1 << 20) * 8]
+        del junk
+        got = layer(qkv, positions, short, weight, weight, 1e-6)
+        with pytest.raises(RuntimeError, match="out-of-range"):
+            check_status(torch.device(DEV))
+        keep = positions < last
+        assert torch.equal(got[keep], want[keep])
+    reset_context()
