@@ -16,7 +16,8 @@ bfloat16 pattern of the group's scale ``s`` with the four low mantissa bits repl
 * ``prefill_attention_int4``    -- ragged causal chunks, on a cached prefix or without.
 
 On CUDA a slot or block id outside the pool is skipped (its keys are not seen) and recorded for
-``check_status``.  A query that sees no key gives zeros.
+``check_status``.  A query that sees no key gives zeros.  Stored values stay below 2^127 in magnitude, V
+that attention reads below 2^100 (weights reach 2^8 before they are divided by their sum), queries below 2^125.
 """
 import torch
 
