@@ -127,3 +127,49 @@ def test_scales_that_float32_does_not_hold_are_refused(scale):
         kv_int4.decode_attention_int4(q, p, p, t, n, scale)
     with pytest.raises(RuntimeError, match="scale"):
         kv_int4.prefill_attention_int4(q, p, p, _i32(0, 1), n, t, scale, 1)
+
+
+def _nan_key_case():
+    """Token 40 of 64 holds NaN in the first group of its K."""
+    kp, vp = (oracle.random_pages(5, 2, 16, 128, s) for s in (1, 2))
+    tables = torch.tensor([[3, 1, 4, 0]], dtype=torch.int32)
+    q = torch.randn(64, 4, 128, generator=torch.Generator().manual_seed(6)).bfloat16()
+    want, mag = oracle.attention(q, kp, vp, [0, 64], [64], tables, 0.09)
+    kp[1][4, 1, 8, 0] = 0x7FC0
+    nan = torch.zeros_like(q, dtype=torch.bool)
+    nan[40:, 2:] = True
+    return q, kp, vp, tables, want, mag, nan
+
+
+@pytest.mark.parametrize("new", [64, 30])
+def test_a_nan_key_breaks_only_the_rows_that_see_it(new):
+    q, kp, vp, tables, want, mag, nan = _nan_key_case()
+    q, want, mag, nan = (x[64 - new:] for x in (q, want, mag, nan))
+    args = (q.to(DEV), _on(kp), _on(vp))
+    for out in (kv_int4.prefill_attention_int4(*args, _i32(0, new), _i32(64), tables.to(DEV), 0.09, new),
+                kv_int4.verify_attention_int4(*args, tables.to(DEV), _i32(64), 0.09, new)):
+        out = out.cpu()
+        assert torch.equal(out.isnan(), nan)
+        assert ((out.double() - want).abs() <= oracle.attention_tolerance(want, mag))[~nan].all()
+
+
+def test_captured_prefill_replays_on_new_lengths_and_tables():
+    nh, nkv, hd, bs, T = 8, 2, 64, 16, 200
+    kp, vp = (oracle.random_pages(20, nkv, bs, hd, s) for s in (1, 2))
+    q = torch.randn(T, nh, hd, generator=torch.Generator().manual_seed(1)).bfloat16()
+    args, cu, lens, tables = (q.to(DEV), _on(kp), _on(vp)), _i32(0, 0, 0, 0), _i32(0, 0, 0), torch.zeros(3, 14, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kv_int4.prefill_attention_int4(*args, cu, lens, tables, 0.125, T)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = kv_int4.prefill_attention_int4(*args, cu, lens, tables, 0.125, T)
+        for seed, (q_lens, k_lens) in enumerate((((130, 1, 69), (200, 90, 69)), ((0, 200, 0), (5, 220, 0)), ((1, 1, 1), (1, 2, 224)))):
+            table = torch.randint(0, 20, (3, 14), generator=torch.Generator().manual_seed(seed)).int()
+            ends = [0, q_lens[0], q_lens[0] + q_lens[1], sum(q_lens)]
+            cu.copy_(_i32(*ends)), lens.copy_(_i32(*k_lens)), tables.copy_(table)
+            graph.replay()
+            side.synchronize()
+            want, mag = oracle.attention(q, kp, vp, ends, k_lens, table, 0.125)
+            _assert_close(out[:ends[-1]], want[:ends[-1]], mag[:ends[-1]])
